@@ -12,6 +12,24 @@ int64_t linear_wgrad(at::Tensor dy, at::Tensor x, at::Tensor out, bool accumulat
                      c10::optional<at::Tensor> npart, int64_t offset);
 void gemm_test(at::Tensor a, bool a_mn, at::Tensor b, bool b_mn, at::Tensor out, int splits);
 void gemm_trace(c10::optional<at::Tensor> buf);
+void cache_write(at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_exp,
+                 c10::optional<at::Tensor> v_exp, at::Tensor k, at::Tensor v, at::Tensor slots);
+std::vector<at::Tensor> cache_read(at::Tensor k_pool, at::Tensor v_pool, c10::optional<at::Tensor> k_exp,
+                                   c10::optional<at::Tensor> v_exp, at::Tensor table, at::Tensor lens,
+                                   c10::optional<at::Tensor> starts, int64_t length);
+std::vector<at::Tensor> tree_attention(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor k_pool, at::Tensor v_pool,
+                                       c10::optional<at::Tensor> k_exp, c10::optional<at::Tensor> v_exp,
+                                       at::Tensor table, at::Tensor lens, at::Tensor parents,
+                                       c10::optional<at::Tensor> counts, c10::optional<at::Tensor> gate,
+                                       c10::optional<double> scale);
+at::Tensor gdn_advance(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor g, at::Tensor beta, at::Tensor state,
+                       int64_t groups, c10::optional<at::Tensor> counts, c10::optional<at::Tensor> rows,
+                       at::Tensor out_state);
+std::vector<at::Tensor> gdn_verify(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor g, at::Tensor beta,
+                                   at::Tensor state, at::Tensor parents, int64_t groups,
+                                   c10::optional<at::Tensor> counts, c10::optional<at::Tensor> rows);
+void gdn_accept(at::Tensor k, at::Tensor g, at::Tensor u, at::Tensor path, at::Tensor state, int64_t groups,
+                c10::optional<at::Tensor> rows, at::Tensor out_state);
 void rms_norm_fwd(at::Tensor x, at::Tensor w, double eps, at::Tensor y, at::Tensor inv);
 void rms_norm_bwd(at::Tensor dy, at::Tensor x, at::Tensor inv, at::Tensor w, at::Tensor dx, at::Tensor dw,
                   c10::optional<at::Tensor> res);
@@ -154,6 +172,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("conv_silu_vec", &ns::conv_silu_vec);
   m.def("head_norm_rope", &ns::head_norm_rope, "(1+w)-RMSNorm per head row + partial RoPE");
   m.def("vattn_fwd", &ns::vattn_fwd, "causal GQA flash attention (tcgen05) with sigmoid output gate");
+  m.def("cache_write", &ns::cache_write, "K/V rows into pages, quantising");
+  m.def("cache_read", &ns::cache_read, "a range of cached positions as bf16");
+  m.def("tree_attention", &ns::tree_attention, "attention of drafted nodes over a paged cache");
+  m.def("gdn_advance", &ns::gdn_advance, "gated delta rule over tokens from a carried state");
+  m.def("gdn_verify", &ns::gdn_verify, "gated delta rule over a tree of nodes");
+  m.def("gdn_accept", &ns::gdn_accept, "state after an accepted path");
   m.def("device_error", &ns::device_error, "read the kernels' bounded-wait error word");
   m.def("clear_device_error", &ns::clear_device_error);
   m.def("device_error_tensor", &ns::device_error_tensor, "the error word as a 1-element int32 CUDA view");

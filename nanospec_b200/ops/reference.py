@@ -459,3 +459,103 @@ def gated_delta_rule_backward(q, k, v, g, beta, dout):
         out = gated_delta_rule_recurrent(*leaves)
         out.backward(dout.float())
     return tuple(t.grad for t in leaves)
+
+
+# ------------------------------------------------------------------------- decoding over a cache
+CACHE_EXP_BIAS, CACHE_EXP_MIN, CACHE_EXP_MAX = 127, -117, 118
+
+
+def cache_encode(x):
+    """Rows [..., D] -> (e4m3 codes, uint8 exponents [...]): code = e4m3(x 2^-e) with the
+    smallest e for which the row's largest finite magnitude is <= 448 * 2^e (clamped to
+    [-117, 118]; 0 for a row of zeros). The exponent byte is e + 127; larger magnitudes and
+    infinities saturate, NaN stays NaN. Both scalings are exact, so only e4m3's own
+    rounding (to nearest even) is lost."""
+    x = x.float()
+    a = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x)).amax(-1)
+    m, e = torch.frexp(a)
+    e = torch.where(m > 0.875, e - 8, e - 9).clamp(CACHE_EXP_MIN, CACHE_EXP_MAX)
+    e = torch.where(a == 0, torch.zeros_like(e), e)
+    y = torch.ldexp(x, -e.unsqueeze(-1))
+    y = torch.where(torch.isnan(y), y, y.clamp(-448, 448))
+    return y.to(torch.float8_e4m3fn), (e + CACHE_EXP_BIAS).to(torch.uint8)
+
+
+def cache_decode(codes, exps):
+    """code * 2^e in fp32 (exact; bf16 holds every value too)."""
+    return torch.ldexp(codes.float(), exps.int().unsqueeze(-1) - CACHE_EXP_BIAS)
+
+
+def tree_ancestors(parents, counts):
+    """[b, T, T] bool: column a is row t itself or one of its ancestors; rows and columns
+    beyond ``counts`` are empty. parents [b, T] (-1: child of the last cached token)."""
+    b, t = parents.shape
+    anc = torch.zeros(b, t, t, dtype=torch.bool, device=parents.device)
+    row = torch.arange(b, device=parents.device)
+    for i in range(t):
+        p = parents[:, i].long()
+        anc[:, i] = anc[row, p.clamp_min(0)] & (p >= 0).unsqueeze(-1)
+        anc[:, i, i] = True
+    live = torch.arange(t, device=parents.device) < counts[:, None]
+    return anc & live[:, :, None] & live[:, None, :]
+
+
+def tree_attention(q, k, v, prefix_k, prefix_v, lens, anc, gate, scale):
+    """Softmax attention of nodes over a per-sequence prefix and their ancestors, fp32.
+
+    q [b, T, Hq, D]; k, v [b, T, Hk, D]; prefix_k/v [b, L, Hk, D] with ``lens`` valid
+    rows each; anc [b, T, T]. Rows that see nothing give zeros and lse -inf.
+    """
+    b, t, hq, d = q.shape
+    g = hq // k.shape[2]
+    live = torch.diagonal(anc, dim1=1, dim2=2)  # [b, T]
+    seen = torch.arange(prefix_k.shape[1], device=q.device) < lens[:, None]
+    zero = torch.zeros((), device=q.device)
+    clean = lambda x, m: torch.where(m[:, :, None, None], x.float(), zero).repeat_interleave(g, 2).transpose(1, 2)  # noqa: E731
+    kk = torch.cat((clean(prefix_k, seen), clean(k, live)), 2)
+    vv = torch.cat((clean(prefix_v, seen), clean(v, live)), 2)
+    see = torch.cat(((live[:, :, None] & seen[:, None, :]), anc), 2)[:, None]
+    s = (q.float().transpose(1, 2) @ kk.transpose(2, 3) * scale).masked_fill(~see, -torch.inf)
+    lse = torch.logsumexp(s, -1)
+    p = torch.exp(s - torch.where(torch.isfinite(lse), lse, zero).unsqueeze(-1))
+    o = (p @ vv).transpose(1, 2)
+    if gate is not None:
+        o = torch.where(live[:, :, None, None], o * torch.sigmoid(gate.float()), zero)
+    return o.to(q.dtype), lse
+
+
+def gated_delta_nodes(q, k, v, g, beta, state, parents, counts):
+    """The gated delta rule over nodes in topological order, fp32: node t starts from the
+    state of parents[:, t] (-1: ``state``). q, k [b, T, h, d] raw (L2-normalised here, q
+    scaled by d^-1/2), v, g, beta per head, state [b, h, d, d]. Returns (out, u, states of
+    the last counted node): u_t = beta_t (v_t - S^T k_t) is the row that node t adds."""
+    dtype = q.dtype
+    q = l2norm(q.float()) * q.shape[-1] ** -0.5
+    k = l2norm(k.float())
+    v, g, beta = v.float(), g.float(), beta.float()
+    b, t = q.shape[:2]
+    out, u, last = torch.zeros_like(v), torch.zeros_like(v), state.clone()
+    for i in range(b):
+        states = {-1: state[i]}
+        chain = bool((parents[i] == torch.arange(-1, t - 1)).all())
+        for n in range(int(counts[i])):
+            s = states[int(parents[i, n])] * g[i, n].exp()[:, None, None]
+            if chain:
+                states.clear()
+            u[i, n] = beta[i, n, :, None] * (v[i, n] - torch.einsum("hkv,hk->hv", s, k[i, n]))
+            s = s + k[i, n, :, :, None] * u[i, n, :, None, :]
+            out[i, n] = torch.einsum("hkv,hk->hv", s, q[i, n])
+            states[n] = s
+            last[i] = s
+    return out.to(dtype), u, last
+
+
+def gated_delta_accept(k, g, u, path, state):
+    """State after the nodes ``path`` [b, m] (-1 skipped), in order: S <- e^g S + k u^T."""
+    k = l2norm(k.float())
+    out = state.clone()
+    for i in range(path.shape[0]):
+        for n in path[i].tolist():
+            if n >= 0:
+                out[i] = out[i] * g[i, n].float().exp()[:, None, None] + k[i, n, :, :, None] * u[i, n, :, None, :]
+    return out

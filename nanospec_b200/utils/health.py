@@ -21,7 +21,8 @@ timeout raises in the same ``train()`` call with the default synchronous
 optimizer, or at the start of the next call otherwise.
 
 Codes: 1 = an mbarrier wait in a tensor-core kernel, 2 = a peer flag wait, 3 = a
-token id outside the embedding table (the kernel skipped the access).
+token id outside the embedding table (the kernel skipped the access), 4 = an index of a
+decoding op (slot, page, length, parent, count, path, row) out of range (skipped).
 Reference policy: the reference raises on schedule misuse
 (nanospec/shard.py:230-231,247-248) and relies on a finite NCCL timeout
 (nanospec/distributed.py:24); it has no device-side waits of its own.
@@ -34,7 +35,8 @@ import torch
 from ..ops._ext import cuda_ops
 
 CODES = {1: "a tensor-core kernel's mbarrier wait", 2: "a peer-memory flag wait",
-         3: "an index out of range in an embedding gather or scatter (the access was skipped)"}
+         3: "an index out of range in an embedding gather or scatter (the access was skipped)",
+         4: "an index out of range in a decoding op (the access was skipped)"}
 
 
 class DeviceWaitTimeout(RuntimeError):
@@ -44,7 +46,7 @@ class DeviceWaitTimeout(RuntimeError):
     def __init__(self, code: int, tag: str):
         self.code, self.tag = code, tag
         what = CODES.get(code, f"error code {code}")
-        verb = "was reported" if code == 3 else "timed out"
+        verb = "was reported" if code in (3, 4) else "timed out"
         super().__init__(f"{what} {verb} on the device during '{tag}'; the step's outputs are invalid "
                          f"(device state was reset)")
 
