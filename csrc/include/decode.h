@@ -39,8 +39,9 @@ inline CacheView check_cache(const at::Tensor& k, const at::Tensor& v, const Opt
   if (c.e4m3) {
     for (const OptTensor* e : {&ke, &ve}) {
       NS_VALUE(e->has_value() && (*e)->scalar_type() == at::kByte && (*e)->device() == k.device() &&
-                   (*e)->sizes() == k.sizes().slice(0, 3) && (*e)->is_contiguous(),
-               "cache: e4m3 pages need uint8 exponents [pages, heads, page_size]");
+                   (*e)->sizes() == k.sizes().slice(0, 3) && (*e)->is_contiguous() &&
+                   reinterpret_cast<uintptr_t>((*e)->data_ptr()) % 16 == 0,
+               "cache: e4m3 pages need aligned uint8 exponents [pages, heads, page_size]");
     }
     c.ke = ke->data_ptr<uint8_t>();
     c.ve = ve->data_ptr<uint8_t>();

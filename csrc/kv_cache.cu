@@ -2,7 +2,8 @@
 //
 // A row x[D] of one (token, head) is kept as bf16, or as e4m3 codes with one power-of-two
 // scale: with a the largest finite |x|, e is the smallest integer for which
-// a <= 448 * 2^e, clamped to [-117, 118] (0 for a row of zeros), and
+// a <= 448 * 2^e, clamped to [-117, 118] (-117 for a row of zeros, so that
+// it never sets the scale of others), and
 //   code = e4m3(x * 2^-e)  (nearest even, saturating, NaN kept),   byte = e + 127,
 //   read  = code * 2^e.
 // Multiplying by a power of two is exact both ways and bf16 holds every code * 2^e, so the
@@ -25,8 +26,7 @@ constexpr int EXP_BIAS = 127, EXP_MIN = -117, EXP_MAX = 118;
 
 // exponent byte of a row whose largest finite magnitude has the fp32 bits `a`
 __device__ __forceinline__ int row_exponent(uint32_t a) {
-  if (a == 0) return 0;
-  const int E = max((int)(a >> 23), 1) - 127;  // bf16 subnormals are far below EXP_MIN
+  const int E = (int)(a >> 23) - 127;  // zero and subnormals are far below EXP_MIN
   const int e = E - 8 + ((a & 0x7fffff) > 0x600000 ? 1 : 0);
   return min(max(e, EXP_MIN), EXP_MAX);
 }

@@ -468,14 +468,14 @@ CACHE_EXP_BIAS, CACHE_EXP_MIN, CACHE_EXP_MAX = 127, -117, 118
 def cache_encode(x):
     """Rows [..., D] -> (e4m3 codes, uint8 exponents [...]): code = e4m3(x 2^-e) with the
     smallest e for which the row's largest finite magnitude is <= 448 * 2^e (clamped to
-    [-117, 118]; 0 for a row of zeros). The exponent byte is e + 127; larger magnitudes and
+    [-117, 118]; -117 for a row of zeros). The exponent byte is e + 127; larger magnitudes and
     infinities saturate, NaN stays NaN. Both scalings are exact, so only e4m3's own
     rounding (to nearest even) is lost."""
     x = x.float()
     a = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x)).amax(-1)
     m, e = torch.frexp(a)
     e = torch.where(m > 0.875, e - 8, e - 9).clamp(CACHE_EXP_MIN, CACHE_EXP_MAX)
-    e = torch.where(a == 0, torch.zeros_like(e), e)
+    e = torch.where(a == 0, torch.full_like(e, CACHE_EXP_MIN), e)
     y = torch.ldexp(x, -e.unsqueeze(-1))
     y = torch.where(torch.isnan(y), y, y.clamp(-448, 448))
     return y.to(torch.float8_e4m3fn), (e + CACHE_EXP_BIAS).to(torch.uint8)
