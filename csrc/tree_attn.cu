@@ -8,10 +8,11 @@
 // and all T nodes, so up to G T = 250 rows or so the tensor cores wait for HBM. So K/V is
 // read once for 128 stacked rows (GT heads x TPM tokens) and one pass keeps the running
 // maximum and sum:
-//   S_j = Q K_j^T      M=128, N=64, K=D -> TMEM (two 64-column buffers)
-//   O  += P_j V_j      M=128, N=D, K=64 -> TMEM, P_j read from TMEM
-// over tiles of 64 keys: the tiles of the cached prefix, then one tile of the nodes' own
-// keys whose mask is the row's ancestor set.
+//   S_j = Q K_j^T      M=128, N=128, K=D -> TMEM (two 128-column buffers)
+//   O  += P_j V_j      M=128, N=D, K=128 -> TMEM, P_j over its own S_j in TMEM
+// over tiles of 128 keys: the tiles of the cached prefix, then one tile of the nodes' own
+// keys whose mask is the row's ancestor set. S_{j+1} is issued before P_j V_j, so the tensor
+// cores work while the softmax warps (two threads per row) form P.
 //
 // Work is split over the long axis without knowing the lengths on the host: the tiles of
 // all segments (sequence, key head, row tile) are numbered through, and CTA i of N (one per
@@ -20,14 +21,18 @@
 // leave unnormalised O with its reference maximum and sum in a workspace (two parts per CTA
 // at most), and tree_join_kernel adds them up in the order of the CTAs.
 //
-// e4m3 pages: raw codes arrive by TMA, two converter warps turn them into f16 operand tiles
-// (exact), and the rows' power-of-two scales stay outside the products: K's multiplies the
-// score, V's the probability, relative to the largest V scale seen so far (when that
-// grows by more than 2^4, O is rescaled like for a growing maximum). q rows are
-// scaled by a power of two each so that f16 holds all of bf16's digits; the nodes' own
-// rows are scaled the same way. Probabilities are f16 (11 bits) there. Against bf16 V they
-// must be bf16, whose 8 bits would cost as much as the output's own rounding, so P is the
-// sum of two bf16 matrices (16 bits) and P V two products: the tensor cores have the time.
+// bf16 pages: P must be bf16 like V, whose 8 bits would cost as much as the output's own
+// rounding, so P is the sum of two bf16 matrices (16 bits) and P V two products.
+//
+// e4m3 pages: the codes of K go to the tensor cores as they are (kind::f8f6f4). q, scaled by
+// a power of two per row, is the sum of an e4m3 and an e5m2 matrix: rounding q's 8
+// significant bits to 4 leaves at most 8 units of the last of them, which the 3 of e5m2 hold
+// exactly (elements below 2^-14 of the row's largest are held to 2^-22 of it). V's codes
+// become f16 in shared memory (converter warps; code bits shifted into place, i.e.
+// value * 2^-8, exact) against f16 probabilities (11 bits). The rows' scales stay outside
+// the products: K's multiplies the score, V's the probability, relative to the largest V scale
+// seen so far (when that grows by more than 2^4, O is rescaled like for a growing
+// maximum). The nodes' own rows get scales of the same kind; their K is split like q.
 //
 // Rows of V beyond a sequence's end (stale pages, NaN) are zeroed in shared memory, since
 // 0 * NaN would reach O; masked scores are replaced, not added to. Every mbarrier wait is
@@ -45,12 +50,12 @@ using bf16 = __nv_bfloat16;
 namespace tattn {
 
 constexpr int EXP_BIAS = 127, EXP_MIN = -117, EXP_MAX = 118;
-constexpr int BM = 128, BN = 64;
+constexpr int BM = 128, BN = 128;
 constexpr float RESCALE_LOG2 = 8.f;   // the reference maximum may lag by this much
 constexpr int V_RESCALE = 4;          // and the reference V exponent by this much
 constexpr float F16_OFFSET = 3.f;     // f16 probabilities are at most 2^(3 + 8 + 4)
-constexpr int FAC = 4;                // scale buffers of the e4m3 form, see below
-constexpr int CONV_WARPS = 4;
+constexpr int SLOT = 16384;           // bytes of one ring slot
+constexpr int SOFT_WARPS = 8, CONV_WARPS = 6;
 
 struct Args {
   const bf16 *q, *k, *v, *gate;
@@ -88,6 +93,13 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* err) {
   return false;
 }
 
+// The same by one lane for its warp (32 lanes polling one barrier queue up on it).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err) {
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) ok = wait(bar, parity, err);
+  return __shfl_sync(0xffffffff, ok, 0);
+}
+
 // ------------------------------------------------------------------ work split
 struct Seq {
   int len, cnt;
@@ -117,6 +129,8 @@ struct Piece {
   int nt;                 // prefix tiles of the segment (0 when no token is live)
   int t0, t1;             // tiles [t0, t1) of [0, nt]; tile nt is the nodes' own
   bool whole;
+  __device__ __forceinline__ int keys(int t) const { return t < nt ? min(BN, q.len - t * BN) : own; }
+  int own;                // keys of the nodes' tile
 };
 
 struct Walk {
@@ -136,6 +150,7 @@ struct Walk {
     p.hb = (seg / a.M) % a.HB;
     p.hk = seg / (a.M * a.HB);
     p.nt = p.m * a.TPM < q.cnt ? (q.len + BN - 1) / BN : 0;
+    p.own = p.m * a.TPM < q.cnt ? q.cnt : 0;
     p.t0 = tile;
     p.t1 = (int)min((int64_t)p.nt + 1, tile + (end - unit));
     p.whole = p.t0 == 0 && p.t1 == p.nt + 1;
@@ -196,31 +211,47 @@ __device__ __forceinline__ Walk plan(const Args& a, int lane, int64_t& U, int& N
 }
 
 // ------------------------------------------------------------------ shared memory
-template <int DT, bool E4M3>
-struct Cfg {
-  static constexpr int DA = DT / 64;               // 128-byte swizzle atoms along D
-  static constexpr int Q_BYTES = BM * DT * 2;
-  static constexpr int SLOT = BN * DT * 2;         // one operand tile (K or V)
-  static constexpr int NS = E4M3 ? 3 : (DT == 256 ? 4 : 8);
-  static constexpr int RAW = BN * DT;              // one tile of codes
-  static constexpr int NR = E4M3 ? (DT == 256 ? 3 : 8) : 0;
-  static constexpr int FACS = E4M3 ? FAC * 2 * BN * 4 + FAC * 16 : 0;
-  static constexpr int EXPS = NR * 2 * BN;
-  static constexpr int SMEM = Q_BYTES + NS * SLOT + NR * RAW + FACS + EXPS + 512 + 1024;
-  static constexpr int PP = E4M3 ? 1 : 2;          // matrices whose sum is P
-  static constexpr int S_COL = DT, P_COL = DT + 2 * BN, P_COLS = PP * (BN / 2);
-  static constexpr int TMEM_COLS = P_COL + 2 * P_COLS <= 256 ? 256 : 512;
-  static constexpr int THREADS = 192 + (E4M3 ? CONV_WARPS * 32 : 0);
-  // Scale buffer of tile n is reused by tile n + FAC, whose K enters ring slot
-  // 2 (n + FAC) - 1; that slot is free once item 2 (n + FAC) - 1 - NS, at or after V of
-  // tile n (item 2n + 2), was consumed, i.e. after tile n's probabilities were formed.
-  static_assert(!E4M3 || 2 * FAC - 1 - NS >= 2, "scale buffers");
+// A ring of 16 KB slots with its position and phase.
+struct Ring {
+  int st = 0, ph = 0;
+  __device__ __forceinline__ void step(int size) {
+    if (++st == size) st = 0, ph ^= 1;
+  }
 };
 
-// Ring items of a piece of n tiles, in the order of the MMAs: K0, (K1, V0), (K2, V1), .., V(n-1).
-// f(tile, is_v) returns false to stop.
+template <int DT, bool E4M3>
+struct Cfg {
+  static constexpr int DA = DT / 64;               // 128-byte swizzle atoms of 16-bit elements along D
+  static constexpr int VK = BN / DA;               // keys in one slot of 16-bit V rows
+  static constexpr int KS = E4M3 ? DT / 128 : DA;  // slots of one K tile
+  static constexpr int RS = E4M3 ? DT / 128 : 0;   // slots of one tile of V codes
+  static constexpr int RK = E4M3 ? BN / (RS + !E4M3) : BN;   // keys in one of them
+  static constexpr int Q_BYTES = BM * DT * 2;      // bf16, or the two 8-bit matrices
+  // Ring sizes (slots). bf16: one ring, K and V in the order of the products. e4m3: K codes,
+  // V codes, f16 V.
+  static constexpr int NK = E4M3 ? 4 : (DT == 256 ? 9 : 11);
+  static constexpr int NR = E4M3 ? (DT == 256 ? 2 : 3) : 0;
+  static constexpr int NV = E4M3 ? (DT == 256 ? 3 : 4) : 0;
+  static constexpr int PP = E4M3 ? 1 : 2;          // matrices whose sum is P
+  static constexpr int XCH = 2 * 2 * 2 * BM * 4;   // maxima and sums exchanged by a row's two threads
+  // e4m3 scales of FAC tiles: exponent bytes, K and V factors, largest V exponent. Buffer n % FAC
+  // is written again for tile n + FAC once that tile has its KS ring slots, the last of which
+  // held tile n + 2 or a later one (NK <= KS (FAC - 2)); and S of tile n + 2 is only issued
+  // after P of tile n was formed.
+  static constexpr int FAC = KS == 2 ? 4 : 8;
+  static constexpr int FACS = E4M3 ? FAC * (2 * BN + 2 * BN * 4 + 16) : 0;
+  static constexpr int SMEM = Q_BYTES + (NK + NR + NV) * SLOT + FACS + XCH + 512 + 1024;
+  static constexpr int S_COL = DT;
+  static constexpr int TMEM_COLS = DT + 2 * BN <= 256 ? 256 : 512;
+  static constexpr int THREADS = 32 * (2 + SOFT_WARPS + (E4M3 ? CONV_WARPS : 0));
+  static_assert(SMEM <= 232448, "shared memory");
+  static_assert(!E4M3 || NK <= KS * (FAC - 2), "scale buffers");
+};
+
+// Tiles of a piece in the order of the products: S0, (S1, PV0), (S2, PV1), .., PV(n-1).
+// f(tile, is_pv) returns false to stop.
 template <class F>
-__device__ __forceinline__ bool ring_order(int t0, int t1, F&& f) {
+__device__ __forceinline__ bool product_order(int t0, int t1, F&& f) {
   if (!f(t0, false)) return false;
   for (int t = t0; t < t1; ++t) {
     if (t + 1 < t1 && !f(t + 1, false)) return false;
@@ -229,22 +260,61 @@ __device__ __forceinline__ bool ring_order(int t0, int t1, F&& f) {
   return true;
 }
 
-// exponent that brings a row with largest magnitude bits `top` into [2^8, 2^9)
-__device__ __forceinline__ int f16_exponent(uint32_t top) {
-  return top == 0 ? EXP_MIN : max(min(max((int)(top >> 23), 1) - 127 - 8, EXP_MAX), EXP_MIN);
+// exponent that brings a row whose largest magnitude has the bits `top` into [2^at, 2^(at+1))
+__device__ __forceinline__ int row_exponent(uint32_t top, int at) {
+  return max(min((int)(top >> 23) - 127 - at, EXP_MAX), EXP_MIN);
 }
 
-__device__ __forceinline__ uint32_t finite_top(uint32_t w) {  // of two packed bf16
-  const uint32_t lo = (w << 16) & 0x7fffffffu, hi = w & 0x7fff0000u;
-  return max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u);
+__device__ __forceinline__ uint32_t finite_top(uint4 w) {  // largest finite magnitude of 8 bf16
+  const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = (in[i] << 16) & 0x7fffffffu, hi = in[i] & 0x7fff0000u;
+    top = max(top, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
+  }
+  return top;
 }
 
-__device__ __forceinline__ uint32_t scale_to_f16(uint32_t w, float s) {  // two packed bf16
-  const __half2 h = __floats2half2_rn(__uint_as_float(w << 16) * s, __uint_as_float(w & 0xffff0000u) * s);
-  return *reinterpret_cast<const uint32_t*>(&h);
+__device__ __forceinline__ uint4 scale_to_f16(uint4 w, float s) {  // 8 bf16
+  uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(__uint_as_float(x[i] << 16) * s, __uint_as_float(x[i] & 0xffff0000u) * s);
+    x[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
-// offset of 16-byte chunk c (8 elements) of row r in a K-major 128-byte-swizzled tile of `rows` rows
+// 8 bf16 times s as the sum of e4m3 and e5m2
+__device__ __forceinline__ void split_fp8(uint4 w, float s, uint2& hi, uint2& lo) {
+  const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+  uint32_t h[2] = {0, 0}, l[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = __uint_as_float(x[i] << 16) * s, b = __uint_as_float(x[i] & 0xffff0000u) * s;
+    const __nv_fp8x2_storage_t c = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(c, __NV_E4M3)));
+    const __nv_fp8x2_storage_t r = __nv_cvt_float2_to_fp8x2(make_float2(a - f.x, b - f.y), __NV_SATFINITE, __NV_E5M2);
+    h[i / 2] |= (uint32_t)c << (16 * (i & 1));
+    l[i / 2] |= (uint32_t)r << (16 * (i & 1));
+  }
+  hi = make_uint2(h[0], h[1]);
+  lo = make_uint2(l[0], l[1]);
+}
+
+// 4 e4m3 codes -> 4 f16 of value * 2^-8: exponent and mantissa bits shifted into place (both
+// formats count subnormals the same way). NaN codes become 1.875 here.
+__device__ __forceinline__ uint2 codes_to_f16(uint32_t w) {
+  const uint32_t a = __byte_perm(w, 0, 0x1404), b = __byte_perm(w, 0, 0x3424);
+  return make_uint2((a & 0x80008000u) | ((a & 0x7f007f00u) >> 1), (b & 0x80008000u) | ((b & 0x7f007f00u) >> 1));
+}
+
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) {  // non-zero if one of 4 codes is NaN
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
+// byte offset of 16-byte chunk c of row r in a K-major 128-byte-swizzled tile of `rows` rows
 __device__ __forceinline__ uint32_t tile_offset(int rows, int r, int c) {
   return (uint32_t)((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
@@ -255,32 +325,36 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
                      const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tkp,
                      const __grid_constant__ CUtensorMap tvp, Args a) {
   using C = Cfg<DT, E4M3>;
-  constexpr int DA = C::DA, NS = C::NS, NR = C::NR;
+  constexpr int DA = C::DA, VK = C::VK, KS = C::KS, NK = C::NK, NR = C::NR, NV = C::NV, FAC = C::FAC;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sQ = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sKV = sQ + C::Q_BYTES;
-  uint8_t* sRaw = sKV + NS * C::SLOT;
-  float* kfac = reinterpret_cast<float*>(sRaw + NR * C::RAW);    // [FAC][BN] 2^e of K rows
-  float* vfac = kfac + (E4M3 ? FAC * BN : 0);                    // [FAC][BN] 2^(e - emax) of V rows
-  int* vmax = reinterpret_cast<int*>(vfac + (E4M3 ? FAC * BN : 0));  // [FAC][4] emax of each tile
-  uint8_t* sExp = reinterpret_cast<uint8_t*>(sRaw + NR * C::RAW + C::FACS);  // [NR][2][BN]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sExp + C::EXPS);
-  uint64_t* full = bars;             // [NS] operand tile ready
-  uint64_t* empty = full + NS;       // [NS]
-  uint64_t* raw_full = empty + NS;   // [NR] codes landed
-  uint64_t* raw_empty = raw_full + NR;
-  uint64_t* fac_full = raw_empty + NR;  // [FAC] (e4m3)
-  uint64_t* s_full = fac_full + (E4M3 ? FAC : 0);
-  uint64_t* s_free = s_full + 2;
-  uint64_t* p_full = s_free + 2;
-  uint64_t* p_free = p_full + 2;
-  uint64_t* q_full = p_free + 2;
+  uint8_t* sK = sQ + C::Q_BYTES;      // [NK] (bf16: K and V)
+  uint8_t* sRaw = sK + NK * SLOT;     // [NR] codes of V
+  uint8_t* sV = E4M3 ? sRaw + NR * SLOT : sK;
+  float* kfac = reinterpret_cast<float*>(sK + (NK + NR + NV) * SLOT);  // [FAC][BN] 2^e of K rows
+  float* vfac = kfac + (E4M3 ? FAC * BN : 0);                          // [FAC][BN] 2^(e - emax) of V rows
+  int* vmax = reinterpret_cast<int*>(vfac + (E4M3 ? FAC * BN : 0));    // [FAC][4] emax of each tile
+  uint8_t* sExp = reinterpret_cast<uint8_t*>(vmax + (E4M3 ? FAC * 4 : 0));  // [FAC][2][BN] exponent bytes
+  float* xmax = reinterpret_cast<float*>(sExp + (E4M3 ? FAC * 2 * BN : 0));  // [2][2][BM]
+  float* xsum = xmax + 2 * 2 * BM;                                           // [2][2][BM]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(xsum + 2 * 2 * BM);
+  uint64_t* k_full = bars;           // [NK]
+  uint64_t* k_empty = k_full + NK;   // [NK]
+  uint64_t* r_full = k_empty + NK;   // [NR]
+  uint64_t* r_empty = r_full + NR;   // [NR]
+  uint64_t* v_full = E4M3 ? r_empty + NR : k_full;   // [NV]
+  uint64_t* v_empty = E4M3 ? v_full + NV : k_empty;  // [NV]
+  uint64_t* e_full = r_empty + NR + 2 * NV;          // [FAC] exponent bytes landed
+  uint64_t* f_full = e_full + (E4M3 ? FAC : 0);      // [FAC] factors ready
+  uint64_t* s_full = f_full + (E4M3 ? FAC : 0);      // [2]
+  uint64_t* p_full = s_full + 2;                     // [2]
+  uint64_t* q_full = p_full + 2;
   uint64_t* q_empty = q_full + 1;
   uint64_t* o_done = q_empty + 1;  // one completion per PV (rescales wait for the previous one)
   uint64_t* o_last = o_done + 1;   // one per piece, after its last PV
   uint64_t* o_free = o_last + 1;   // one per piece, O has been read
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 1);
-  static_assert(2 * NS + 2 * NR + FAC + 13 + 1 <= 64, "barrier area");
+  static_assert(2 * (NK + NR + NV + FAC) + 9 + 1 <= 64, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int64_t U;
@@ -289,26 +363,16 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
   if (walk.unit >= walk.end) return;
 
   if (warp == 0 && lane == 0) {
-    for (int i = 0; i < NS; ++i) {
-      sm100::mbar_init(&full[i], E4M3 ? CONV_WARPS : 1);
-      sm100::mbar_init(&empty[i], 1);
-    }
-    for (int i = 0; i < NR; ++i) {
-      sm100::mbar_init(&raw_full[i], 1);
-      sm100::mbar_init(&raw_empty[i], CONV_WARPS);
-    }
-    for (int i = 0; i < (E4M3 ? FAC : 0); ++i) sm100::mbar_init(&fac_full[i], CONV_WARPS);
-    for (int i = 0; i < 2; ++i) {
-      sm100::mbar_init(&s_full[i], 1);
-      sm100::mbar_init(&s_free[i], 4);
-      sm100::mbar_init(&p_full[i], 4);
-      sm100::mbar_init(&p_free[i], 1);
-    }
-    sm100::mbar_init(q_full, E4M3 ? 4 : 1);
+    for (int i = 0; i < NK; ++i) sm100::mbar_init(&k_full[i], 1), sm100::mbar_init(&k_empty[i], 1);
+    for (int i = 0; i < NR; ++i) sm100::mbar_init(&r_full[i], 1), sm100::mbar_init(&r_empty[i], CONV_WARPS);
+    for (int i = 0; i < NV; ++i) sm100::mbar_init(&v_full[i], CONV_WARPS), sm100::mbar_init(&v_empty[i], 1);
+    for (int i = 0; i < (E4M3 ? FAC : 0); ++i) sm100::mbar_init(&e_full[i], 1), sm100::mbar_init(&f_full[i], 1);
+    for (int i = 0; i < 2; ++i) sm100::mbar_init(&s_full[i], 1), sm100::mbar_init(&p_full[i], SOFT_WARPS);
+    sm100::mbar_init(q_full, E4M3 ? SOFT_WARPS : 1);
     sm100::mbar_init(q_empty, 1);
     sm100::mbar_init(o_done, 1);
     sm100::mbar_init(o_last, 1);
-    sm100::mbar_init(o_free, 4);
+    sm100::mbar_init(o_free, SOFT_WARPS);
     sm100::fence_barrier_init();
     sm100::tma_prefetch_desc(&tkp);
     sm100::tma_prefetch_desc(&tvp);
@@ -321,195 +385,307 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int br = min(a.page, BN);  // rows of one page that one copy brings
-
-  // pool row of key `key` of a sequence (a page out of range is replaced by page 0)
-  auto pool_row = [&](const Piece& p, int key) -> int {
-    int pg = __ldg(a.table + p.s * a.max_pages + key / a.page);
-    if (pg < 0 || pg >= a.pages) {
-      atomicExch(a.err, ERR_INDEX);
-      pg = 0;
-    }
-    return (pg * a.Hk + p.hk) * a.page + key % a.page;
-  };
 
   Piece p;
   if (warp == 0) {
-    // ---------------------------------------------------------- TMA producer
-    if (lane == 0) {
-      int it = 0, pc = 0;
-      bool ok = true;
-      while (ok && walk.next(a, p)) {
-        if constexpr (!E4M3) {
-          if (pc > 0 && !(ok = wait(q_empty, (pc - 1) & 1, a.err))) break;
-          sm100::mbar_expect_tx(q_full, DA * a.GT * a.TPM * 128);
-#pragma unroll
-          for (int j = 0; j < DA; ++j)
-            sm100::tma_load_4d(sQ + j * (BM * 128), &tq, q_full, 64 * j, p.hk * a.G + p.hb * a.GT, p.m * a.TPM, p.s);
-          ++pc;
+    // ---------------------------------------------------------- TMA producer, a copy per lane
+    constexpr int VR = E4M3 ? C::RK : VK;  // keys of one slot of the pages' V rows
+    constexpr int VA = E4M3 ? DT / 64 : DA;
+    const int kb = min(a.page, BN), vb = min(a.page, VR);  // rows that one copy brings
+    Ring kr, rr;
+    int n = 0, pc = 0;
+    bool ok = true;
+    while (ok && walk.next(a, p)) {
+      if constexpr (!E4M3) {
+        if (pc > 0 && !(ok = warp_wait(q_empty, (pc - 1) & 1, a.err))) break;
+        if (lane == 0) sm100::mbar_expect_tx(q_full, DA * a.GT * a.TPM * 128);
+        __syncwarp();
+        if (lane < DA)
+          sm100::tma_load_4d(sQ + lane * (BM * 128), &tq, q_full, 64 * lane, p.hk * a.G + p.hb * a.GT, p.m * a.TPM,
+                             p.s);
+        ++pc;
+      }
+      // pool row of 16 keys (lane l: keys 16 l ..) of tile t; a page out of range is replaced by page 0
+      auto rows16 = [&](int t) -> int {
+        const int key = t * BN + (lane & 7) * 16;
+        if (t >= p.nt || key >= p.q.len) return 0;
+        int pg = __ldg(a.table + p.s * a.max_pages + key / a.page);
+        if (pg < 0 || pg >= a.pages) {
+          atomicExch(a.err, ERR_INDEX);
+          pg = 0;
         }
-        ok = ring_order(p.t0, p.t1, [&](int t, bool is_v) -> bool {
-          constexpr int R = E4M3 ? NR : NS;
-          const int st = it % R, use = it / R;
-          uint64_t* fb = E4M3 ? &raw_full[st] : &full[st];
-          if (t == p.nt) {  // the nodes' own rows (the e4m3 form reads them in the converters)
-            if constexpr (!E4M3) {
-              if (use > 0 && !wait(&empty[st], (use - 1) & 1, a.err)) return false;
-              uint8_t* d = sKV + st * C::SLOT;
-              sm100::mbar_expect_tx(fb, DA * a.T * 128);
-#pragma unroll
-              for (int j = 0; j < DA; ++j)
-                sm100::tma_load_4d(d + j * (BN * 128), is_v ? &tv : &tk, fb, 64 * j, p.hk, 0, p.s);
-              ++it;
+        return (pg * a.Hk + p.hk) * a.page + key % a.page;
+      };
+      // of the last S tile, the one before it (whose PV follows), the next one (read ahead)
+      int row_s = 0, row_p = 0, row_n = rows16(p.t0);
+      ok = product_order(p.t0, p.t1, [&](int t, bool pv) -> bool {
+        const int keys = p.keys(t);
+        const bool own = t == p.nt;
+        if (!pv) {
+          row_p = row_s;
+          row_s = row_n;
+          if (t + 1 < p.t1) row_n = rows16(t + 1);
+          const int runs = (keys + kb - 1) / kb;
+#pragma unroll 1
+          for (int j = 0; j < KS; ++j) {
+            if (E4M3 && own) {  // the converters fill these
+              kr.step(NK);
+              continue;
             }
-            return true;
+            if (!warp_wait(&k_empty[kr.st], kr.ph ^ 1, a.err)) return false;
+            uint64_t* fb = &k_full[kr.st];
+            uint8_t* d = sK + kr.st * SLOT;
+            if (own) {
+              if (lane == 0) {
+                sm100::mbar_expect_tx(fb, a.T * 128);
+                sm100::tma_load_4d(d, &tk, fb, 64 * j, p.hk, 0, p.s);
+              }
+            } else {
+              if (lane == 0) sm100::mbar_expect_tx(fb, runs * kb * 128);
+              __syncwarp();
+              const int row = __shfl_sync(0xffffffff, row_s, lane * kb / 16 & 7);
+              if (lane < runs) sm100::tma_load_2d(d + lane * kb * 128, &tkp, fb, (E4M3 ? 128 : 64) * j, row);
+            }
+            __syncwarp();
+            kr.step(NK);
           }
-          if (use > 0 && !wait(E4M3 ? &raw_empty[st] : &empty[st], (use - 1) & 1, a.err)) return false;
-          const int k0 = t * BN, n = min(BN, p.q.len - k0), runs = (n + br - 1) / br;
           if constexpr (E4M3) {
-            uint8_t* d = sRaw + st * C::RAW;
-            sm100::mbar_expect_tx(fb, runs * br * (DA * 64 + (is_v ? 0 : 2)));
-            for (int r = 0; r < runs; ++r) {
-              const int row = pool_row(p, k0 + r * br);
+            if (!own) {
+              uint64_t* eb = &e_full[n % FAC];
+              if (lane == 0) sm100::mbar_expect_tx(eb, runs * kb * 2);
+              __syncwarp();
+              const int row = __shfl_sync(0xffffffff, row_s, (lane >> 1) * kb / 16 & 7);
+              if (lane < 2 * runs)
+                sm100::bulk_load(sExp + ((n % FAC) * 2 + (lane & 1)) * BN + (lane >> 1) * kb,
+                                 ((lane & 1) ? a.ve : a.ke) + row, kb, eb);
+              __syncwarp();
+            }
+            ++n;
+          }
+        } else {
+          const int rows = t + 1 < p.t1 ? row_p : row_s;
+          Ring& r = E4M3 ? rr : kr;
+#pragma unroll 1
+          for (int i = 0; i * VR < keys; ++i) {
+            if (E4M3 && own) continue;
+            if (!warp_wait(E4M3 ? &r_empty[r.st] : &k_empty[r.st], r.ph ^ 1, a.err)) return false;
+            uint64_t* fb = E4M3 ? &r_full[r.st] : &k_full[r.st];
+            uint8_t* d = (E4M3 ? sRaw : sK) + r.st * SLOT;
+            constexpr int ROW = E4M3 ? 64 : 128;  // bytes of a row in one column block
+            if (own) {
+              if (lane == 0) sm100::mbar_expect_tx(fb, DA * min(a.T, VK) * 128);
+              __syncwarp();
+              if (lane < DA) sm100::tma_load_4d(d + lane * (VK * 128), &tv, fb, 64 * lane, p.hk, i * VK, p.s);
+            } else {
+              const int runs = (min(VR, keys - i * VR) + vb - 1) / vb;
+              if (lane == 0) sm100::mbar_expect_tx(fb, VA * runs * vb * ROW);
+              __syncwarp();
 #pragma unroll
-              for (int j = 0; j < DA; ++j)
-                sm100::tma_load_2d(d + j * (BN * 64) + r * br * 64, is_v ? &tvp : &tkp, fb, 64 * j, row);
-              if (!is_v) {
-                sm100::bulk_load(sExp + (st * 2) * BN + r * br, a.ke + row, br, fb);
-                sm100::bulk_load(sExp + (st * 2 + 1) * BN + r * br, a.ve + row, br, fb);
+              for (int x0 = 0; x0 < VA * (VR / 16); x0 += 32) {  // lanes over column blocks x runs
+                const int x = x0 + lane, j = x % VA, u = x / VA;
+                const int row = __shfl_sync(0xffffffff, rows, (i * VR + u * vb) / 16 & 7);
+                if (u < runs)
+                  sm100::tma_load_2d(d + j * (VR * ROW) + u * vb * ROW, &tvp, fb, 64 * j, row);
               }
             }
-          } else {
-            uint8_t* d = sKV + st * C::SLOT;
-            sm100::mbar_expect_tx(fb, runs * br * DA * 128);
-            for (int r = 0; r < runs; ++r) {
-              const int row = pool_row(p, k0 + r * br);
-#pragma unroll
-              for (int j = 0; j < DA; ++j)
-                sm100::tma_load_2d(d + j * (BN * 128) + r * br * 128, is_v ? &tvp : &tkp, fb, 64 * j, row);
-            }
+            __syncwarp();
+            r.step(E4M3 ? NR : NK);
           }
-          ++it;
-          return true;
-        });
-      }
-      // drain: every issued copy has landed before the CTA may exit
-      constexpr int R = E4M3 ? NR : NS;
-      if (!E4M3 && pc > 0) wait(q_full, (pc - 1) & 1, a.err);
-      for (int i = max(0, it - R); i < it; ++i)
-        wait(E4M3 ? &raw_full[i % R] : &full[i % R], (i / R) & 1, a.err);
+        }
+        return true;
+      });
+    }
+    // drain: every issued copy has landed before the CTA may exit
+    if (!E4M3 && pc > 0) warp_wait(q_full, (pc - 1) & 1, a.err);
+    for (int i = 0; i < NK; ++i) {  // slots that were never armed count as empty
+      warp_wait(&k_empty[kr.st], kr.ph ^ 1, a.err);
+      kr.step(NK);
+    }
+    for (int i = 0; i < NR; ++i) {
+      warp_wait(&r_empty[rr.st], rr.ph ^ 1, a.err);
+      rr.step(NR);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
-    constexpr uint32_t idesc_s = E4M3 ? sm100::idesc_f16(BM, BN, false, false) : sm100::idesc_bf16(BM, BN, false, false);
     constexpr uint32_t idesc_o = E4M3 ? sm100::idesc_f16(BM, DT, false, true) : sm100::idesc_bf16(BM, DT, false, true);
     const uint32_t q_base = sm100::smem_u32(sQ);
-    int it = 0, n = 0, ns = 0, pc = 0;  // ring item, PV tile, S tile, piece
+    Ring kr, vr;
+    int n = 0, ns = 0, pc = 0;  // PV tile, S tile, piece
     bool ok = true;
     while (ok && walk.next(a, p)) {
-      ok = wait(q_full, pc & 1, a.err);
-      ok = ok && ring_order(p.t0, p.t1, [&](int t, bool is_v) -> bool {
-        const int st = it % NS;
-        if (!wait(&full[st], (it / NS) & 1, a.err)) return false;
-        uint8_t* tile = sKV + st * C::SLOT;
-        const uint32_t base = sm100::smem_u32(tile);
-        if (!is_v) {
-          const int sb = ns & 1;
-          if (ns >= 2 && !wait(&s_free[sb], ((ns >> 1) - 1) & 1, a.err)) return false;
-          sm100::tc_fence_after();
-          if (lane == 0) {
-#pragma unroll
-            for (int kk = 0; kk < DT / 16; ++kk) {
-              const uint64_t ad = sm100::smem_desc_sw128(q_base + (kk >> 2) * (BM * 128) + (kk & 3) * 32, 0, 1024);
-              const uint64_t bd = sm100::smem_desc_sw128(base + (kk >> 2) * (BN * 128) + (kk & 3) * 32, 0, 1024);
-              sm100::mma_bf16(tmem + C::S_COL + sb * BN, ad, bd, idesc_s, kk > 0 ? 1u : 0u);
+      ok = warp_wait(q_full, pc & 1, a.err);
+      ok = ok && product_order(p.t0, p.t1, [&](int t, bool pv) -> bool {
+        const int keys = p.keys(t);
+        const bool own = t == p.nt;
+        if (!pv) {
+          // the buffer's last reader, and every product before it, is done
+          if (n > 0 && !warp_wait(o_done, (n - 1) & 1, a.err)) return false;
+          const uint32_t cols = max(16, (keys + 15) & ~15);
+          const uint32_t idesc = sm100::idesc_bf16(BM, 16, false, false) - (2u << 17) + ((cols >> 3) << 17);
+          const uint32_t idesc8 = idesc & ~((1u << 7) | (1u << 10));  // e4m3 x e4m3; bits 7 / 10: e5m2
+          const uint32_t d = tmem + C::S_COL + (ns & 1) * BN;
+          if constexpr (E4M3) {
+            if (own) {  // (Q hi + Q lo) (K hi + K lo), the two K matrices of 64 rows one after the other
+              const uint32_t k_at[2] = {sm100::smem_u32(sK + kr.st * SLOT),
+                                        sm100::smem_u32(sK + (DT == 256 ? (kr.st + 1) % NK : kr.st) * SLOT) +
+                                            (DT == 256 ? 0 : MAX_NODES * 128)};
+              for (int j = 0; j < KS; ++j) {
+                if (!warp_wait(&k_full[kr.st], kr.ph, a.err)) return false;
+                kr.step(NK);
+              }
+              sm100::tc_fence_after();
+              if (lane == 0) {
+                for (int x = 0; x < 4; ++x)
+                  for (int kk = 0; kk < DT / 32; ++kk) {
+                    const uint32_t off = (kk & 3) * 32, at = kk >> 2;
+                    sm100::mma_f8(d, sm100::smem_desc_sw128(q_base + (x & 1) * (BM * DT) + at * (BM * 128) + off, 0, 1024),
+                           sm100::smem_desc_sw128(k_at[x >> 1] + at * (MAX_NODES * 128) + off, 0, 1024),
+                           idesc8 | (x & 1) << 7 | (x >> 1) << 10,
+                           x + kk > 0 ? 1u : 0u);
+                  }
+                for (int j = 0; j < KS; ++j) sm100::mma_commit(&k_empty[(kr.st + NK - 1 - j) % NK]);
+              }
+              __syncwarp();
             }
-            sm100::mma_commit(&s_full[sb]);
-            sm100::mma_commit(&empty[st]);
+          }
+          if (!E4M3 || !own) {
+#pragma unroll 1
+            for (int j = 0; j < KS; ++j) {
+              if (!warp_wait(&k_full[kr.st], kr.ph, a.err)) return false;
+              sm100::tc_fence_after();
+              if (lane == 0) {
+                const uint32_t base = sm100::smem_u32(sK + kr.st * SLOT);
+                if constexpr (E4M3) {
+#pragma unroll
+                  for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                      sm100::mma_f8(d, sm100::smem_desc_sw128(q_base + x * (BM * DT) + j * (BM * 128) + kk * 32, 0, 1024),
+                             sm100::smem_desc_sw128(base + kk * 32, 0, 1024), idesc8 | x << 7,
+                             j + x + kk > 0 ? 1u : 0u);
+                } else {
+#pragma unroll
+                  for (int kk = 0; kk < 4; ++kk)
+                    sm100::mma_bf16(d, sm100::smem_desc_sw128(q_base + j * (BM * 128) + kk * 32, 0, 1024),
+                                    sm100::smem_desc_sw128(base + kk * 32, 0, 1024), idesc, j + kk > 0 ? 1u : 0u);
+                }
+                sm100::mma_commit(&k_empty[kr.st]);
+              }
+              __syncwarp();
+              kr.step(NK);
+            }
+          }
+          if (lane == 0) {
+            sm100::mma_commit(&s_full[ns & 1]);
             if (t == p.t1 - 1) sm100::mma_commit(q_empty);
           }
           __syncwarp();
           ++ns;
         } else {
-          if constexpr (!E4M3) {  // rows of V beyond the end: stale or another sequence's
-            const int live = t == p.nt ? p.q.cnt : min(BN, p.q.len - t * BN);
-            if (live < BN) {
-              for (int i = lane; i < (BN - live) * 8 * DA; i += 32) {
-                const int r = live + i / (8 * DA), c = i % (8 * DA);
-                *reinterpret_cast<uint4*>(tile + tile_offset(BN, r, c)) = make_uint4(0, 0, 0, 0);
-              }
-              sm100::fence_proxy_async_smem();
-              __syncwarp();
-            }
-          }
           const int pb = n & 1;
-          if (!wait(&p_full[pb], (n >> 1) & 1, a.err)) return false;
-          if (t == p.t0 && pc > 0 && !wait(o_free, (pc - 1) & 1, a.err)) return false;
-          sm100::tc_fence_after();
-          if (lane == 0) {
-#pragma unroll
-            for (int kk = 0; kk < C::PP * (BN / 16); ++kk) {
-              const uint64_t bd = sm100::smem_desc_sw128(base + (kk % (BN / 16)) * 2048, BN * 128, 1024);
-              sm100::mma_f16_ts(tmem, tmem + C::P_COL + pb * C::P_COLS + kk * 8, bd, idesc_o,
-                                (t > p.t0 || kk > 0) ? 1u : 0u);
+          bool have_p = false;
+#pragma unroll 1
+          for (int i = 0; i * VK < keys; ++i) {
+            Ring& r = E4M3 ? vr : kr;
+            if (!warp_wait(&v_full[r.st], r.ph, a.err)) return false;
+            uint8_t* tile = sV + r.st * SLOT;
+            const int live = min(VK, keys - i * VK);
+            if constexpr (!E4M3) {  // rows of V beyond the end, up to the next product's edge
+              if (live & 15) {
+                const int dead = 16 - (live & 15);
+                for (int x = lane; x < dead * 8 * DA; x += 32)
+                  *reinterpret_cast<uint4*>(tile + tile_offset(VK, live + x / (8 * DA), x % (8 * DA))) =
+                      make_uint4(0, 0, 0, 0);
+                sm100::fence_proxy_async_smem();
+                __syncwarp();
+              }
             }
+            if (!have_p) {
+              if (!warp_wait(&p_full[pb], (n >> 1) & 1, a.err)) return false;
+              if (t == p.t0 && pc > 0 && !warp_wait(o_free, (pc - 1) & 1, a.err)) return false;
+              have_p = true;
+            }
+            sm100::tc_fence_after();
+            if (lane == 0) {
+              const uint32_t base = sm100::smem_u32(tile), ps = tmem + C::S_COL + pb * BN;
+              for (int kk = 0; kk * 16 < live; ++kk) {
+                const int k16 = i * (VK / 16) + kk;  // P of 16 keys: 8 columns of its half's 64
+                const uint64_t bd = sm100::smem_desc_sw128(base + kk * 2048, VK * 128, 1024);
+#pragma unroll
+                for (int x = 0; x < C::PP; ++x)
+                  sm100::mma_f16_ts(tmem, ps + (k16 >> 2) * 64 + x * 32 + (k16 & 3) * 8, bd, idesc_o,
+                                    (t > p.t0 || k16 + x > 0) ? 1u : 0u);
+              }
+              sm100::mma_commit(&v_empty[r.st]);
+            }
+            __syncwarp();
+            r.step(E4M3 ? NV : NK);
+          }
+          if (!have_p) {  // no keys at all: O is not read
+            if (!warp_wait(&p_full[pb], (n >> 1) & 1, a.err)) return false;
+            if (t == p.t0 && pc > 0 && !warp_wait(o_free, (pc - 1) & 1, a.err)) return false;
+          }
+          if (lane == 0) {
             sm100::mma_commit(o_done);
             if (t == p.t1 - 1) sm100::mma_commit(o_last);
-            sm100::mma_commit(&p_free[pb]);
-            sm100::mma_commit(&empty[st]);
           }
           __syncwarp();
           ++n;
         }
-        ++it;
         return true;
       });
       ++pc;
     }
-  } else if (warp < 6) {
-    // ---------------------------------------------------------- softmax warps, one row per thread
-    const int qw = warp & 3;  // TMEM lane quarter of this warp
+  } else if (warp < 2 + SOFT_WARPS) {
+    // ---------------------------------------------------------- softmax warps
+    // Two threads per row, each with 64 of a tile's 128 scores and half of O's columns. They
+    // exchange their maxima through shared memory. No early exit: a warp whose wait ran out
+    // (ok = false) keeps meeting its partner at the barriers, only without further waits.
+    const int qw = warp & 3, half = (warp - 2) >> 2;  // TMEM lane quarter, column half
     const int row = qw * 32 + lane;
     const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
     const int rows = a.GT * a.TPM;
     const bool warp_on = qw * 32 < rows;
     int n = 0, pc = 0;
     bool ok = true;
-    while (ok && walk.next(a, p)) {
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) { ok = ok && warp_wait(bar, parity, a.err); };
+    auto exchange = [&](float* buf, float v) -> float {  // the partner's value
+      buf[half * BM + row] = v;
+      sm100::named_sync(1 + qw, 64);
+      return buf[(half ^ 1) * BM + row];
+    };
+    while (walk.next(a, p)) {
       const int tok = p.m * a.TPM + row / a.GT, g = p.hb * a.GT + row % a.GT;
       const bool in = row < rows && g < a.G && tok < a.T;
       const bool live = in && tok < p.q.cnt;
       const int hq = p.hk * a.G + g;
       float rs = a.scale_log2;  // multiplies the products of this row
       if constexpr (E4M3) {
-        // q row -> f16 with a power-of-two scale, into the operand tile (the previous piece's
-        // products are complete: this thread has seen all of its scores)
+        // q row -> e4m3 and e5m2 rows with a power-of-two scale (the previous piece's products are
+        // complete: this thread has seen all of its scores)
         if (live) {
           const bf16* q = a.q + p.s * a.q_bs + tok * a.q_ts + hq * a.q_hs;
           uint32_t top = 0;
-          for (int c = 0; c < a.D / 8; ++c) {
-            const uint4 w = *reinterpret_cast<const uint4*>(q + c * 8);
-            top = max(max(max(top, finite_top(w.x)), max(finite_top(w.y), finite_top(w.z))), finite_top(w.w));
-          }
-          const int e = f16_exponent(top);
-          const float s = pow2(-e);
+#pragma unroll 4
+          for (int c = 0; c < a.D / 8; ++c) top = max(top, finite_top(*reinterpret_cast<const uint4*>(q + c * 8)));
+          const int e = row_exponent(top, 7);
           rs *= pow2(e);
-          for (int c = 0; c < DT / 8; ++c) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (c * 8 < a.D) {
-              w = *reinterpret_cast<const uint4*>(q + c * 8);
-              w = make_uint4(scale_to_f16(w.x, s), scale_to_f16(w.y, s), scale_to_f16(w.z, s), scale_to_f16(w.w, s));
-            }
-            *reinterpret_cast<uint4*>(sQ + tile_offset(BM, row, c)) = w;
+#pragma unroll 2
+          for (int c = half * (DT / 16); c < (half + 1) * (DT / 16); ++c) {
+            uint2 hi = make_uint2(0, 0), lo = make_uint2(0, 0);
+            if (c * 8 < a.D) split_fp8(*reinterpret_cast<const uint4*>(q + c * 8), pow2(-e), hi, lo);
+            const uint32_t at = tile_offset(BM, row, c >> 1) + (c & 1) * 8;
+            *reinterpret_cast<uint2*>(sQ + at) = hi;
+            *reinterpret_cast<uint2*>(sQ + BM * DT + at) = lo;
           }
         }
         sm100::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(q_full);
       }
-      // ancestors of this row's node
+      // ancestors of this row's node (all in the first half's columns)
       uint64_t anc = 0;
-      if (live && p.t1 == p.nt + 1) {
+      if (live && half == 0 && p.t1 == p.nt + 1) {
         for (int i = tok; i >= 0;) {
           anc |= 1ull << i;
           int up = a.parents[p.s * a.p_bs + i];
@@ -520,93 +696,79 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
           i = up;
         }
       }
-      float m = -INFINITY, l = 0.f;  // reference maximum (log2) and sum
+      float m = -INFINITY, l = 0.f;  // reference maximum (log2) and this half's sum
       int ev = 0;                    // reference exponent of V (e4m3)
       for (int t = p.t0; t < p.t1; ++t, ++n) {
-        const int sb = n & 1;
-        const uint64_t mask = !live ? 0ull
-                              : t == p.nt ? anc
-                              : p.q.len - t * BN >= BN ? ~0ull
-                                                       : (1ull << (p.q.len - t * BN)) - 1;
-        ok = __all_sync(0xffffffff, wait(&s_full[sb], (n >> 1) & 1, a.err));
-        if (E4M3 && ok) ok = __all_sync(0xffffffff, wait(&fac_full[n % FAC], (n / FAC) & 1, a.err));
-        if (!ok) break;
+        const int sb = n & 1, left = p.keys(t) - half * 64;
+        const uint64_t mask = t == p.nt ? anc : left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+        wait_all(&s_full[sb], (n >> 1) & 1);
+        if constexpr (E4M3) wait_all(&f_full[n % FAC], (n / FAC) & 1);
         sm100::tc_fence_after();
-        const float* kf = kfac + (n % FAC) * BN;
-        const float* vf = vfac + (n % FAC) * BN;
-        float x[BN];
-        if (warp_on) {
-          float tmp[32];
-#pragma unroll
-          for (int hlf = 0; hlf < 2; ++hlf) {
-            sm100::tmem_ld32(tmem + lane_off + C::S_COL + sb * BN + hlf * 32, tmp);
-#pragma unroll
-            for (int c = 0; c < 32; ++c) x[hlf * 32 + c] = tmp[c];
-          }
-        }
-        sm100::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&s_free[sb]);
-        float alpha = 1.f, alpha_o = 1.f;
+        float alpha_o = 1.f;
         bool grow = false;
-        uint32_t pk[BN / 2];
-        if (warp_on) {
-          float mt = -INFINITY;
+        const uint32_t scol = tmem + lane_off + C::S_COL + sb * BN + half * 64;
+        const float* kf = kfac + (n % FAC) * BN + half * 64;
+        const float* vf = vfac + (n % FAC) * BN + half * 64;
+        // 32 scores: read, K's scale (e4m3), mask
+        auto scores = [&](int c0, float (&x)[32]) {
+          sm100::tmem_ld32(scol + c0, x);
+          if constexpr (E4M3) {
 #pragma unroll
-          for (int c = 0; c < BN; ++c) x[c] = E4M3 ? x[c] * (rs * kf[c]) : x[c] * rs;
-          if (mask != ~0ull) {
-#pragma unroll
-            for (int c = 0; c < BN; ++c)
-              if (!((mask >> c) & 1)) x[c] = -INFINITY;
+            for (int c = 0; c < 32; c += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(kf + c0 + c);
+              x[c] *= f.x, x[c + 1] *= f.y, x[c + 2] *= f.z, x[c + 3] *= f.w;
+            }
           }
+          const uint32_t mk = (uint32_t)(mask >> c0);
+          if (mk != 0xffffffffu) {
 #pragma unroll
-          for (int c = 0; c < BN; ++c) mt = fmaxf(mt, x[c]);
-          const float top = E4M3 ? mt - F16_OFFSET : mt;
-          if (top > m + RESCALE_LOG2) {
-            alpha = alpha_o = sm100::exp2_approx(m - top);  // 0 on the first tile
+            for (int c = 0; c < 32; ++c)
+              if (!(mk & (1u << c))) x[c] = -INFINITY;
+          }
+        };
+        auto largest = [&](const float (&x)[32]) -> float {
+          float mx[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = x[i];
+#pragma unroll
+          for (int c = 4; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
+          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        };
+        float x[E4M3 ? 1 : 2][32];  // the e4m3 form has fewer registers and reads them again
+        if (warp_on) {
+          scores(0, x[0]);
+          float mt = largest(x[0]);
+          scores(32, x[C::PP - 1]);
+          mt = fmaxf(mt, largest(x[C::PP - 1]));
+          mt = fmaxf(mt, exchange(xmax + sb * 2 * BM, mt));
+          const float top = mt * rs - (E4M3 ? F16_OFFSET : 0.f);
+          if (live && top > m + RESCALE_LOG2) {
+            alpha_o = sm100::exp2_approx(m - top);  // 0 on the first tile
+            l *= alpha_o;
             m = top;
             grow = true;
           }
-          const float ref = m == -INFINITY ? 0.f : m;
-          float vs = 1.f;
-          if constexpr (E4M3) {
-            const int e = vmax[(n % FAC) * 4];
-            if (t == p.t0) ev = e;
-            if (e > ev + V_RESCALE) {
-              alpha_o *= pow2(max(ev - e, -126));
-              ev = e;
-              grow = true;
-            }
-            vs = pow2(max(e - ev, -126));
-          }
-          float ps = 0.f;
-#pragma unroll
-          for (int c = 0; c < BN; c += 2) {
-            const float p0 = sm100::exp2_approx(x[c] - ref), p1 = sm100::exp2_approx(x[c + 1] - ref);
-            ps += p0 + p1;
-            x[c] = p0, x[c + 1] = p1;
-            if constexpr (E4M3) {
-              const __half2 h2 = __floats2half2_rn(p0 * (vs * vf[c]), p1 * (vs * vf[c + 1]));
-              pk[c / 2] = *reinterpret_cast<const uint32_t*>(&h2);
-            } else {
-              const __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
-              pk[c / 2] = *reinterpret_cast<const uint32_t*>(&h2);
-            }
-          }
-          l = l * alpha + ps;
         }
-        // the P buffer is free once PV of tile n - 2 completed
-        if (n >= 2) {
-          ok = __all_sync(0xffffffff, wait(&p_free[sb], ((n >> 1) - 1) & 1, a.err));
-          if (!ok) break;
+        float ref = m == -INFINITY ? 0.f : m, back = 1.f;
+        if constexpr (E4M3) {
+          const int e = vmax[(n % FAC) * 4];
+          if (t == p.t0) ev = e;
+          if (e > ev + V_RESCALE) {
+            alpha_o *= pow2(max(ev - e, -126));
+            ev = e;
+            grow = true;
+          }
+          // this tile's V scale relative to the reference goes into the exponent
+          const int de = max(e - ev, -100);
+          ref -= (float)de;
+          back = pow2(-de);
         }
         // rescale O rows once the previous PV completed (warp-wide, rare after the first tiles)
-        if (__any_sync(0xffffffff, grow && t > p.t0)) {
-          ok = __all_sync(0xffffffff, wait(o_done, (n - 1) & 1, a.err));
-          if (!ok) break;
+        if (__any_sync(0xffffffff, warp_on && grow && t > p.t0)) {
+          wait_all(o_done, (n - 1) & 1);
           sm100::tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < DT; c += 32) {
+          for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32) {
             float o[32];
             sm100::tmem_ld32(tmem + lane_off + c, o);
 #pragma unroll
@@ -615,31 +777,52 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
           }
         }
         if (warp_on) {
-          float f[32];
+          float ps[2] = {0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(pk[i]);
-          sm100::tmem_st32(tmem + lane_off + C::P_COL + sb * C::P_COLS, f);
-          if constexpr (!E4M3) {  // what the first rounding left
+          for (int h = 0; h < 2; ++h) {
+            uint32_t hi[16], lo[16];
+            if constexpr (E4M3) scores(h * 32, x[0]);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const __nv_bfloat162 h2 = __floats2bfloat162_rn(x[2 * i] - __uint_as_float(pk[i] << 16),
-                                                              x[2 * i + 1] - __uint_as_float(pk[i] & 0xffff0000u));
-              f[i] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&h2));
+            for (int c = 0; c < 32; c += 4) {
+              float pr[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) pr[i] = sm100::exp2_approx(fmaf(x[h * (C::PP - 1)][c + i], rs, -ref));
+              ps[0] += pr[0] + pr[1];
+              ps[1] += pr[2] + pr[3];
+              if constexpr (E4M3) {
+                const float4 f = *reinterpret_cast<const float4*>(vf + h * 32 + c);
+                const __half2 h0 = __floats2half2_rn(pr[0] * f.x, pr[1] * f.y);
+                const __half2 h1 = __floats2half2_rn(pr[2] * f.z, pr[3] * f.w);
+                hi[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
+                hi[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                  const __nv_bfloat162 h2 = __floats2bfloat162_rn(pr[i], pr[i + 1]);
+                  const uint32_t w = *reinterpret_cast<const uint32_t*>(&h2);
+                  const __nv_bfloat162 l2 = __floats2bfloat162_rn(pr[i] - __uint_as_float(w << 16),
+                                                                  pr[i + 1] - __uint_as_float(w & 0xffff0000u));
+                  hi[(c + i) / 2] = w;
+                  lo[(c + i) / 2] = *reinterpret_cast<const uint32_t*>(&l2);
+                }
+              }
             }
-            sm100::tmem_st32(tmem + lane_off + C::P_COL + sb * C::P_COLS + BN / 2, f);
+            sm100::tmem_st16_async(scol + h * 16, hi);  // over this thread's own scores
+            if constexpr (!E4M3) sm100::tmem_st16_async(scol + 32 + h * 16, lo);
           }
+          l += (ps[0] + ps[1]) * back;
+          sm100::tmem_st_wait();
         }
         sm100::tc_fence_before();
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(&p_full[sb]);
       }
-      if (!ok) break;
-      ok = __all_sync(0xffffffff, wait(o_last, pc & 1, a.err));
-      if (!ok) break;
+      wait_all(o_last, pc & 1);
       sm100::tc_fence_after();
       if (warp_on) {
+        l += exchange(xsum + (pc & 1) * 2 * BM, l);
         // O -> the output (a whole segment) or the workspace
-        const float vs = E4M3 ? pow2(ev) : 1.f;
+        const float vs = E4M3 ? pow2(ev + 8) : 1.f;
         const float inv = l > 0.f ? vs / l : (l == 0.f ? 0.f : l);
         // the piece a CTA begins in the middle of its run starts a segment and ends the run
         const int slot = p.t0 == 0 && walk.end - (p.t1 - p.t0) != U * blockIdx.x / N ? 1 : 0;
@@ -647,7 +830,7 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
         bf16* o = a.out + (((int64_t)p.s * a.T + tok) * a.Hq + hq) * a.D;
         const bf16* gt = a.gate ? a.gate + p.s * a.g_bs + tok * a.g_ts + hq * a.g_hs : nullptr;
 #pragma unroll 1
-        for (int c = 0; c < DT; c += 32) {
+        for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32) {
           float v[32];
           sm100::tmem_ld32(tmem + lane_off + c, v);
           if (!in) continue;
@@ -679,14 +862,14 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
                          : make_float4(0.f, 0.f, 0.f, 0.f);
           }
         }
-        if (in) {
+        if (in && half == 0) {
           if (p.whole)
             a.lse[((int64_t)p.s * a.Hq + hq) * a.T + tok] =
                 live ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
           else
-            a.ml[at] = make_float2(m, l);
+            a.ml[at] = live ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
         }
-        if (row == 0 && p.t0 == 0) {  // where the segment's parts are
+        if (row == 0 && half == 0 && p.t0 == 0) {  // where the segment's parts are
           const int64_t first = walk.unit - (p.t1 - p.t0), last = first + p.nt;
           const int c1 = (int)(((last + 1) * N - 1) / U);
           a.info[(((int64_t)p.s * a.Hk + p.hk) * a.HB + p.hb) * a.M + p.m] = make_int4(blockIdx.x, c1, slot, 0);
@@ -698,99 +881,153 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
       ++pc;
     }
   } else if constexpr (E4M3) {
-    // ---------------------------------------------------------- converters: codes -> f16 operand tiles
-    const int cw = warp - 6;
-    const int r8 = lane >> 2, q4 = lane & 3;  // row of 8, 16 codes of 64
-    int it = 0, ri = 0, n = 0;
+    // ---------------------------------------------------------- converters
+    // Per tile: the scales' factors (and, for the nodes' own tile, K as two matrices) in
+    // the place of S, V's f16 rows in the place of PV.
+    const int cw = warp - 2 - SOFT_WARPS;
+    Ring kr, rr, vr;
+    int n = 0;
     bool ok = true;
+    // 16-byte chunk of a node's row, and the exponent that brings the row into [2^at, 2^(at+1))
+    auto node_row = [&](const bf16* x, int at, uint4& w) -> int {
+      w = make_uint4(0, 0, 0, 0);
+      if (lane * 8 < a.D) w = *reinterpret_cast<const uint4*>(x + lane * 8);
+      return row_exponent(__reduce_max_sync(0xffffffff, finite_top(w)), at);
+    };
     while (ok && walk.next(a, p)) {
-      ok = ring_order(p.t0, p.t1, [&](int t, bool is_v) -> bool {
-        const int st = it % NS, use = it / NS;
+      ok = product_order(p.t0, p.t1, [&](int t, bool pv) -> bool {
+        const int keys = p.keys(t);
         const bool own = t == p.nt;
-        const int live = own ? p.q.cnt : min(BN, p.q.len - t * BN);
-        const int rst = ri % max(NR, 1);
-        if (!own && !wait(&raw_full[rst], (ri / max(NR, 1)) & 1, a.err)) return false;
-        if (use > 0 && !wait(&empty[st], (use - 1) & 1, a.err)) return false;
-        uint8_t* tile = sKV + st * C::SLOT;
-        const int fb = n % FAC;
-        if (own) {
-          // one row per warp pass: exponent from its largest magnitude, then scaled to f16
-          const bf16* src = is_v ? a.v + p.s * a.v_bs + p.hk * a.v_hs : a.k + p.s * a.k_bs + p.hk * a.k_hs;
-          const int64_t ts = is_v ? a.v_ts : a.k_ts;
-          auto row_exp = [&](const bf16* x, uint4& w) {
-            w = make_uint4(0, 0, 0, 0);
-            if (lane * 8 < a.D) w = *reinterpret_cast<const uint4*>(x + lane * 8);
-            uint32_t top = max(max(finite_top(w.x), finite_top(w.y)), max(finite_top(w.z), finite_top(w.w)));
-            return f16_exponent(__reduce_max_sync(0xffffffff, top));
-          };
-          for (int r = cw; r < BN; r += CONV_WARPS) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            int e = EXP_MIN;
-            if (r < live) {
-              e = row_exp(src + r * ts, w);
-              const float s = pow2(-e);
-              w = make_uint4(scale_to_f16(w.x, s), scale_to_f16(w.y, s), scale_to_f16(w.z, s), scale_to_f16(w.w, s));
+        const bf16* nv = a.v + p.s * a.v_bs + p.hk * a.v_hs;
+        if (!pv) {
+          const int fb = n % FAC;
+          if (own) {
+            const Ring k0 = kr;
+            for (int j = 0; j < KS; ++j) {
+              if (!warp_wait(&k_empty[kr.st], kr.ph ^ 1, a.err)) return false;
+              kr.step(NK);
             }
-            if (lane < DT / 8) *reinterpret_cast<uint4*>(tile + tile_offset(BN, r, lane)) = w;
-            if (!is_v && lane == 0) kfac[fb * BN + r] = pow2(e);
+            uint8_t* hi_at = sK + k0.st * SLOT;
+            uint8_t* lo_at = DT == 256 ? sK + ((k0.st + 1) % NK) * SLOT : hi_at + MAX_NODES * 128;
+            for (int r = cw; r < MAX_NODES; r += CONV_WARPS) {
+              uint4 w = make_uint4(0, 0, 0, 0);
+              int e = EXP_MIN;
+              if (r < keys) e = node_row(a.k + p.s * a.k_bs + p.hk * a.k_hs + r * a.k_ts, 7, w);
+              uint2 hi, lo;
+              split_fp8(w, pow2(-e), hi, lo);
+              if (lane < DT / 8) {
+                const uint32_t at = tile_offset(MAX_NODES, r, lane >> 1) + (lane & 1) * 8;
+                *reinterpret_cast<uint2*>(hi_at + at) = hi;
+                *reinterpret_cast<uint2*>(lo_at + at) = lo;
+              }
+              if (lane == 0) kfac[fb * BN + r] = r < keys ? pow2(e) : 0.f;
+            }
+            sm100::fence_proxy_async_smem();
+            sm100::named_sync(5, CONV_WARPS * 32);
+            if (cw == 0) {
+              if (lane == 0) {
+                sm100::mbar_arrive(&k_full[k0.st]);
+                if (KS == 2) sm100::mbar_arrive(&k_full[(k0.st + 1) % NK]);
+              }
+              // V: the largest exponent, then every row's relative to it
+              int top = EXP_MIN, mine[2] = {EXP_MIN, EXP_MIN};
+              uint4 w;
+              for (int r = 0; r < keys; ++r) {
+                const int e = node_row(nv + r * a.v_ts, 8, w);
+                top = max(top, e);
+                if ((r & 31) == lane) mine[r >> 5] = e;
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                vfac[fb * BN + i * 32 + lane] = i * 32 + lane < keys ? pow2(max(mine[i & 1] - top, -126)) : 0.f;
+#pragma unroll
+              for (int i = 2; i < 4; ++i) kfac[fb * BN + i * 32 + lane] = 0.f;
+              __syncwarp();
+              if (lane == 0) {
+                vmax[fb * 4] = top;
+                sm100::mbar_arrive(&e_full[fb]);  // keeps its phase in step with the tiles
+                sm100::mbar_arrive(&f_full[fb]);
+              }
+            }
+          } else {
+            for (int j = 0; j < KS; ++j) kr.step(NK);
+            if (cw == n % CONV_WARPS) {
+              if (!warp_wait(&e_full[fb], (n / FAC) & 1, a.err)) return false;
+              const uint8_t* ex = sExp + fb * 2 * BN;
+              int e[4], top = EXP_MIN;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int r = lane + 32 * i;
+                kfac[fb * BN + r] = r < keys ? pow2(min(max((int)ex[r] - EXP_BIAS, EXP_MIN), EXP_MAX)) : 0.f;
+                e[i] = min(max((int)ex[BN + r] - EXP_BIAS, EXP_MIN), EXP_MAX);
+                if (r < keys) top = max(top, e[i]);
+              }
+              top = __reduce_max_sync(0xffffffff, top);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                vfac[fb * BN + lane + 32 * i] = lane + 32 * i < keys ? pow2(max(e[i] - top, -126)) : 0.f;
+              if (lane == 0) vmax[fb * 4] = top;
+              __syncwarp();
+              if (lane == 0) sm100::mbar_arrive(&f_full[fb]);
+            }
           }
-          if (!is_v) {  // V's scales: every warp finds the largest, then writes its own rows
-            int top = EXP_MIN, mine = EXP_MIN;
-            uint4 w;
-            for (int r = 0; r < live; ++r) {
-              const int e = row_exp(a.v + p.s * a.v_bs + p.hk * a.v_hs + r * a.v_ts, w);
-              top = max(top, e);
-              if (r % CONV_WARPS == cw && r / CONV_WARPS == lane) mine = e;
+          ++n;
+        } else if (own) {
+          for (int i = 0; i * VK < keys; ++i) {
+            if (!warp_wait(&v_empty[vr.st], vr.ph ^ 1, a.err)) return false;
+            uint8_t* tile = sV + vr.st * SLOT;
+            for (int r = cw; r < min(VK, (keys - i * VK + 15) & ~15); r += CONV_WARPS) {
+              uint4 w = make_uint4(0, 0, 0, 0);
+              if (i * VK + r < keys) {
+                const int e = node_row(nv + (i * VK + r) * a.v_ts, 8, w);
+                w = scale_to_f16(w, pow2(-8 - e));  // value * 2^-8 like the codes
+              }
+              if (lane < DT / 8) *reinterpret_cast<uint4*>(tile + tile_offset(VK, r, lane)) = w;
             }
-            const int r = lane * CONV_WARPS + cw;
-            if (r < BN) vfac[fb * BN + r] = r < live ? pow2(max(mine - top, -126)) : 0.f;
-            if (cw == 0 && lane == 0) vmax[fb * 4] = top;
+            sm100::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&v_full[vr.st]);
+            vr.step(NV);
           }
         } else {
-          const uint8_t* raw = sRaw + rst * C::RAW;
-          for (int i = cw; i < DA * (BN / 8); i += CONV_WARPS) {
-            const int j = i / (BN / 8), r = (i % (BN / 8)) * 8 + r8;
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (r < live) w = *reinterpret_cast<const uint4*>(raw + j * (BN * 64) + r * 64 + q4 * 16);
-            const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-            uint32_t h[8];
+          const int r8 = lane >> 2, q4 = lane & 3;  // row of 8, 16 codes of 64
+          for (int i = 0; i * VK < keys; ++i) {
+            constexpr int PER = C::RK / VK;  // f16 slots that one slot of codes fills
+            if (i % PER == 0 && !warp_wait(&r_full[rr.st], rr.ph, a.err)) return false;
+            if (!warp_wait(&v_empty[vr.st], vr.ph ^ 1, a.err)) return false;
+            const uint8_t* raw = sRaw + rr.st * SLOT + (i % PER) * VK * 64;
+            uint8_t* tile = sV + vr.st * SLOT;
+#pragma unroll 4
+            for (int x = cw; x < DA * (VK / 8); x += CONV_WARPS) {  // 8 rows x 64 channels at a time
+              const int j = x % DA, r = (x / DA) * 8 + r8;
+              uint4 w = *reinterpret_cast<const uint4*>(raw + j * (C::RK * 64) + r * 64 + q4 * 16);
+              if (i * VK + r >= keys) w = make_uint4(0, 0, 0, 0);
+              const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+              uint2 h[4];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const __half2_raw hr =
-                  __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((in[x / 2] >> (16 * (x & 1))) & 0xffff), __NV_E4M3);
-              h[x] = (uint32_t)hr.x | ((uint32_t)hr.y << 16);
+              for (int y = 0; y < 4; ++y) h[y] = codes_to_f16(in[y]);
+              if ((nan_codes(w.x) | nan_codes(w.y)) | (nan_codes(w.z) | nan_codes(w.w))) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                  const uint32_t z = nan_codes(in[y]) >> 7;  // 1 in the byte of each NaN
+                  h[y].x |= ((z & 1) | ((z & 0x100) << 8)) * 0x7fffu;
+                  h[y].y |= (((z >> 16) & 1) | ((z >> 16 & 0x100) << 8)) * 0x7fffu;
+                }
+              }
+              const int c = j * 8 + q4 * 2;
+              *reinterpret_cast<uint4*>(tile + tile_offset(VK, r, c)) = make_uint4(h[0].x, h[0].y, h[1].x, h[1].y);
+              *reinterpret_cast<uint4*>(tile + tile_offset(VK, r, c + 1)) = make_uint4(h[2].x, h[2].y, h[3].x, h[3].y);
             }
-            const int c = j * 8 + q4 * 2;
-            *reinterpret_cast<uint4*>(tile + tile_offset(BN, r, c)) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4*>(tile + tile_offset(BN, r, c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
-          }
-          if (!is_v && cw == 0) {  // this tile's scales, two rows per lane
-            const uint8_t* ex = sExp + rst * 2 * BN;
-            int e[2], top = EXP_MIN;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int r = lane + 32 * i;
-              kfac[fb * BN + r] = r < live ? pow2(min(max((int)ex[r] - EXP_BIAS, EXP_MIN), EXP_MAX)) : 0.f;
-              e[i] = min(max((int)ex[BN + r] - EXP_BIAS, EXP_MIN), EXP_MAX);
-              if (r < live) top = max(top, e[i]);
+            sm100::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              sm100::mbar_arrive(&v_full[vr.st]);
+              if (i % PER == PER - 1 || (i + 1) * VK >= keys) sm100::mbar_arrive(&r_empty[rr.st]);
             }
-            top = __reduce_max_sync(0xffffffff, top);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              vfac[fb * BN + lane + 32 * i] = lane + 32 * i < live ? pow2(max(e[i] - top, -126)) : 0.f;
-            if (lane == 0) vmax[fb * 4] = top;
+            if (i % PER == PER - 1 || (i + 1) * VK >= keys) rr.step(NR);
+            vr.step(NV);
           }
         }
-        sm100::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          sm100::mbar_arrive(&full[st]);
-          if (!own) sm100::mbar_arrive(&raw_empty[rst]);
-          if (!is_v) sm100::mbar_arrive(&fac_full[fb]);
-        }
-        if (!own) ++ri;
-        if (!is_v) ++n;
-        ++it;
         return true;
       });
     }
@@ -871,29 +1108,32 @@ CUtensorMap node_map(const at::Tensor& x, int heads, int tokens) {
   return map;
 }
 
-// Tensor map over the pages as [rows][D]: 64 channels x `rows` box; codes unswizzled.
-CUtensorMap pool_map(const void* base, const CacheView& c, int rows) {
+// Tensor map over the pages as [rows][D], box `cols` x `rows`.
+CUtensorMap pool_map(const void* base, const CacheView& c, int cols, int rows) {
   const int64_t n = c.pages * c.heads * c.page;
-  if (!c.e4m3) return make_tmap_bf16(base, n, c.d, c.d, rows, 64);
+  if (!c.e4m3) return make_tmap_bf16(base, n, c.d, c.d, rows, cols);
   CUtensorMap map;
   cuuint64_t dims[2] = {(cuuint64_t)c.d, (cuuint64_t)n}, strides[1] = {(cuuint64_t)c.d};
-  cuuint32_t box[2] = {64, (cuuint32_t)rows}, estr[2] = {1, 1};
+  cuuint32_t box[2] = {(cuuint32_t)cols, (cuuint32_t)rows}, estr[2] = {1, 1};
   CUresult r = encode_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   NS_CHECK(r == CUDA_SUCCESS, "tree_attention: cuTensorMapEncodeTiled failed");
   return map;
 }
 
 template <int DT, bool E4M3>
-void launch(const Args& a, int grid, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-            const CUtensorMap& tkp, const CUtensorMap& tvp) {
+void launch(const Args& a, int grid, const CacheView& c, const at::Tensor& q, const at::Tensor& k,
+            const at::Tensor& v) {
   using C = Cfg<DT, E4M3>;
-  static_assert(C::SMEM <= 232448, "shared memory");
   static std::atomic<unsigned long long> attr{0};
   once_per_device(attr, [&] {
     NS_CUDA(cudaFuncSetAttribute(tree_attn_kernel<DT, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
   });
+  const CUtensorMap tq = node_map(q, a.GT, a.TPM), tk = node_map(k, 1, a.T), tv = node_map(v, 1, std::min(a.T, C::VK)),
+                    tkp = pool_map(c.k, c, E4M3 ? 128 : 64, std::min(c.page, BN)),
+                    tvp = pool_map(c.v, c, 64, std::min(c.page, E4M3 ? C::RK : C::VK));
   tree_attn_kernel<DT, E4M3><<<grid, C::THREADS, C::SMEM, stream()>>>(tq, tk, tv, tkp, tvp, a);
   NS_CUDA(cudaGetLastError());
 }
@@ -977,19 +1217,13 @@ std::vector<at::Tensor> tree_attention(at::Tensor q, at::Tensor k, at::Tensor v,
   a.part = ws.data_ptr<float>();
   a.ml = reinterpret_cast<float2*>(a.part + n_part);
   a.info = reinterpret_cast<int4*>(a.part + n_part + ((n_ml + 3) & ~int64_t(3)));
-  const int br = std::min(c.page, tattn::BN);
-  const CUtensorMap tq = tattn::node_map(q, a.GT, a.TPM), tk = tattn::node_map(k, 1, (int)T),
-                    tv = tattn::node_map(v, 1, (int)T), tkp = tattn::pool_map(c.k, c, br),
-                    tvp = tattn::pool_map(c.v, c, br);
-#define NS_X(DT)                                                   \
-  {                                                                \
-    if (c.e4m3)                                                    \
-      tattn::launch<DT, true>(a, grid, tq, tk, tv, tkp, tvp);      \
-    else                                                           \
-      tattn::launch<DT, false>(a, grid, tq, tk, tv, tkp, tvp);     \
-  }
-  if (D <= 64) NS_X(64) else if (D <= 128) NS_X(128) else NS_X(256)
-#undef NS_X
+  // the narrowest tile that holds D; e4m3 operands are at least 128 wide (one swizzle atom)
+  if (c.e4m3)
+    D <= 128 ? tattn::launch<128, true>(a, grid, c, q, k, v) : tattn::launch<256, true>(a, grid, c, q, k, v);
+  else if (D <= 64)
+    tattn::launch<64, false>(a, grid, c, q, k, v);
+  else
+    D <= 128 ? tattn::launch<128, false>(a, grid, c, q, k, v) : tattn::launch<256, false>(a, grid, c, q, k, v);
   const int64_t nrows = b * T * Hq;
   tattn::tree_join_kernel<<<(unsigned)((nrows + 7) / 8), 256, 0, stream()>>>(a);
   NS_CUDA(cudaGetLastError());
