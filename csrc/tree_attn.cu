@@ -63,7 +63,7 @@ struct Args {
   const uint8_t *ke, *ve;
   const int *table, *lens, *parents, *counts;
   int64_t p_bs, pages, max_pages;
-  int b, T, Hq, Hk, D, page;
+  int b, T, Hq, Hk, D, page, page_log2;
   int G, GT, HB, TPM, M;  // heads of a group, per row tile, head blocks; tokens per row tile, token blocks
   float scale_log2;
   bf16* out;    // [b, T, Hq, D]
@@ -77,27 +77,23 @@ struct Args {
 __device__ __forceinline__ float bf(bf16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126..127
 
-// Bounded wait: gives up after two seconds (a lost arrival), sets the error word.
+// Bounded wait: gives up after two seconds (a lost arrival), sets the error word. One lane
+// waits for its warp (32 lanes polling one barrier queue up on it); a wait that ran out makes
+// its later waits and products void (`ok`), and every role still walks to its end, so
+// no other wait of the CTA is left without a partner for longer than its own limit.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* err) {
-  if (sm100::mbar_try_wait(bar, parity)) return true;
-  uint64_t t0, t1;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-  for (uint32_t i = 1; i < (1u << 26); ++i) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 1; i < (1u << 28); ++i) {
     if (sm100::mbar_try_wait(bar, parity)) return true;
-    if ((i & 63) == 0) {
-      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
-      if (t1 - t0 > 2000000000ull) break;
+    if ((i & 255) == 0) {
+      uint64_t now;
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+      if (t0 == 0) t0 = now;
+      if (now - t0 > 2000000000ull) break;
     }
   }
   atomicExch(err, 1);
   return false;
-}
-
-// The same by one lane for its warp (32 lanes polling one barrier queue up on it).
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err) {
-  int ok = 1;
-  if ((threadIdx.x & 31) == 0) ok = wait(bar, parity, err);
-  return __shfl_sync(0xffffffff, ok, 0);
 }
 
 // ------------------------------------------------------------------ work split
@@ -240,7 +236,7 @@ struct Cfg {
   // after P of tile n was formed.
   static constexpr int FAC = KS == 2 ? 4 : 8;
   static constexpr int FACS = E4M3 ? FAC * (2 * BN + 2 * BN * 4 + 16) : 0;
-  static constexpr int SMEM = Q_BYTES + (NK + NR + NV) * SLOT + FACS + XCH + 512 + 1024;
+  static constexpr int SMEM = Q_BYTES + (NK + NR + NV) * SLOT + FACS + XCH + 128 + 512 + 1024;
   static constexpr int S_COL = DT;
   static constexpr int TMEM_COLS = DT + 2 * BN <= 256 ? 256 : 512;
   static constexpr int THREADS = 32 * (2 + SOFT_WARPS + (E4M3 ? CONV_WARPS : 0));
@@ -249,15 +245,13 @@ struct Cfg {
 };
 
 // Tiles of a piece in the order of the products: S0, (S1, PV0), (S2, PV1), .., PV(n-1).
-// f(tile, is_pv) returns false to stop.
 template <class F>
-__device__ __forceinline__ bool product_order(int t0, int t1, F&& f) {
-  if (!f(t0, false)) return false;
+__device__ __forceinline__ void product_order(int t0, int t1, F&& f) {
+  f(t0, false);
   for (int t = t0; t < t1; ++t) {
-    if (t + 1 < t1 && !f(t + 1, false)) return false;
-    if (!f(t, true)) return false;
+    if (t + 1 < t1) f(t + 1, false);
+    f(t, true);
   }
-  return true;
 }
 
 // exponent that brings a row whose largest magnitude has the bits `top` into [2^at, 2^(at+1))
@@ -337,7 +331,8 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
   uint8_t* sExp = reinterpret_cast<uint8_t*>(vmax + (E4M3 ? FAC * 4 : 0));  // [FAC][2][BN] exponent bytes
   float* xmax = reinterpret_cast<float*>(sExp + (E4M3 ? FAC * 2 * BN : 0));  // [2][2][BM]
   float* xsum = xmax + 2 * 2 * BM;                                           // [2][2][BM]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(xsum + 2 * 2 * BM);
+  int* page_rows = reinterpret_cast<int*>(xsum + 2 * 2 * BM);                // [4][8] of the producer
+  uint64_t* bars = reinterpret_cast<uint64_t*>(page_rows + 32);
   uint64_t* k_full = bars;           // [NK]
   uint64_t* k_empty = k_full + NK;   // [NK]
   uint64_t* r_full = k_empty + NK;   // [NR]
@@ -388,259 +383,260 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
 
   Piece p;
   if (warp == 0) {
-    // ---------------------------------------------------------- TMA producer, a copy per lane
+    // ---------------------------------------------------------- TMA producer
+    // The whole warp waits; one elected lane issues (ptxas then keeps the operands uniform).
     constexpr int VR = E4M3 ? C::RK : VK;  // keys of one slot of the pages' V rows
     constexpr int VA = E4M3 ? DT / 64 : DA;
+    constexpr int ROW = E4M3 ? 64 : 128;   // bytes of such a row in one column block
     const int kb = min(a.page, BN), vb = min(a.page, VR);  // rows that one copy brings
     Ring kr, rr;
     int n = 0, pc = 0;
     bool ok = true;
-    while (ok && walk.next(a, p)) {
-      if constexpr (!E4M3) {
-        if (pc > 0 && !(ok = warp_wait(q_empty, (pc - 1) & 1, a.err))) break;
-        if (lane == 0) sm100::mbar_expect_tx(q_full, DA * a.GT * a.TPM * 128);
-        __syncwarp();
-        if (lane < DA)
-          sm100::tma_load_4d(sQ + lane * (BM * 128), &tq, q_full, 64 * lane, p.hk * a.G + p.hb * a.GT, p.m * a.TPM,
-                             p.s);
-        ++pc;
-      }
-      // pool row of 16 keys (lane l: keys 16 l ..) of tile t; a page out of range is replaced by page 0
-      auto rows16 = [&](int t) -> int {
-        const int key = t * BN + (lane & 7) * 16;
-        if (t >= p.nt || key >= p.q.len) return 0;
-        int pg = __ldg(a.table + p.s * a.max_pages + key / a.page);
+    // pool rows of 16 keys each (lane l: keys 16 l ..) of tile t, kept in shared memory for the
+    // issuing lane: a page out of range is replaced by page 0
+    auto look_up = [&](int t) {
+      const int key = t * BN + lane * 16;
+      if (lane < 8 && t < p.nt && key < p.q.len) {
+        int pg = __ldg(a.table + p.s * a.max_pages + (key >> a.page_log2));
         if (pg < 0 || pg >= a.pages) {
           atomicExch(a.err, ERR_INDEX);
           pg = 0;
         }
-        return (pg * a.Hk + p.hk) * a.page + key % a.page;
-      };
-      // of the last S tile, the one before it (whose PV follows), the next one (read ahead)
-      int row_s = 0, row_p = 0, row_n = rows16(p.t0);
-      ok = product_order(p.t0, p.t1, [&](int t, bool pv) -> bool {
+        page_rows[(t & 3) * 8 + lane] = ((pg * a.Hk + p.hk) << a.page_log2) + (key & (a.page - 1));
+      }
+      __syncwarp();
+    };
+    while (walk.next(a, p)) {
+      look_up(p.t0);
+      if constexpr (!E4M3) {
+        if (pc > 0) ok = ok && wait(q_empty, (pc - 1) & 1, a.err);
+        if (sm100::elect_one() && ok) {
+          sm100::mbar_expect_tx(q_full, DA * a.GT * a.TPM * 128);
+#pragma unroll
+          for (int j = 0; j < DA; ++j)
+            sm100::tma_load_4d(sQ + j * (BM * 128), &tq, q_full, 64 * j, p.hk * a.G + p.hb * a.GT, p.m * a.TPM, p.s);
+        }
+        __syncwarp();
+        ++pc;
+      }
+      product_order(p.t0, p.t1, [&](int t, bool pv) {
         const int keys = p.keys(t);
         const bool own = t == p.nt;
+        const int* rows = page_rows + (t & 3) * 8;
         if (!pv) {
-          row_p = row_s;
-          row_s = row_n;
-          if (t + 1 < p.t1) row_n = rows16(t + 1);
           const int runs = (keys + kb - 1) / kb;
+          if (t + 1 < p.t1) look_up(t + 1);
+          if (E4M3 && own) {  // the converters fill these
+            for (int j = 0; j < KS; ++j) kr.step(NK);
+          } else {
 #pragma unroll 1
-          for (int j = 0; j < KS; ++j) {
-            if (E4M3 && own) {  // the converters fill these
-              kr.step(NK);
-              continue;
-            }
-            if (!warp_wait(&k_empty[kr.st], kr.ph ^ 1, a.err)) return false;
-            uint64_t* fb = &k_full[kr.st];
-            uint8_t* d = sK + kr.st * SLOT;
-            if (own) {
-              if (lane == 0) {
-                sm100::mbar_expect_tx(fb, a.T * 128);
-                sm100::tma_load_4d(d, &tk, fb, 64 * j, p.hk, 0, p.s);
+            for (int j = 0; j < KS; ++j) {
+              ok = ok && wait(&k_empty[kr.st], kr.ph ^ 1, a.err);
+              if (sm100::elect_one() && ok) {
+                uint64_t* fb = &k_full[kr.st];
+                uint8_t* d = sK + kr.st * SLOT;
+                if (own) {
+                  sm100::mbar_expect_tx(fb, a.T * 128);
+                  sm100::tma_load_4d(d, &tk, fb, 64 * j, p.hk, 0, p.s);
+                } else {
+                  sm100::mbar_expect_tx(fb, runs * kb * 128);
+                  for (int r = 0; r < runs; ++r)
+                    sm100::tma_load_2d(d + r * kb * 128, &tkp, fb, (E4M3 ? 128 : 64) * j, rows[r * kb / 16]);
+                }
               }
-            } else {
-              if (lane == 0) sm100::mbar_expect_tx(fb, runs * kb * 128);
               __syncwarp();
-              const int row = __shfl_sync(0xffffffff, row_s, lane * kb / 16 & 7);
-              if (lane < runs) sm100::tma_load_2d(d + lane * kb * 128, &tkp, fb, (E4M3 ? 128 : 64) * j, row);
+              kr.step(NK);
             }
-            __syncwarp();
-            kr.step(NK);
           }
           if constexpr (E4M3) {
             if (!own) {
-              uint64_t* eb = &e_full[n % FAC];
-              if (lane == 0) sm100::mbar_expect_tx(eb, runs * kb * 2);
-              __syncwarp();
-              const int row = __shfl_sync(0xffffffff, row_s, (lane >> 1) * kb / 16 & 7);
-              if (lane < 2 * runs)
-                sm100::bulk_load(sExp + ((n % FAC) * 2 + (lane & 1)) * BN + (lane >> 1) * kb,
-                                 ((lane & 1) ? a.ve : a.ke) + row, kb, eb);
+              if (sm100::elect_one() && ok) {
+                uint64_t* eb = &e_full[n % FAC];
+                sm100::mbar_expect_tx(eb, runs * kb * 2);
+                for (int r = 0; r < runs; ++r) {
+                  sm100::bulk_load(sExp + (n % FAC) * 2 * BN + r * kb, a.ke + rows[r * kb / 16], kb, eb);
+                  sm100::bulk_load(sExp + ((n % FAC) * 2 + 1) * BN + r * kb, a.ve + rows[r * kb / 16], kb, eb);
+                }
+              }
               __syncwarp();
             }
             ++n;
           }
-        } else {
-          const int rows = t + 1 < p.t1 ? row_p : row_s;
+        } else if (!E4M3 || !own) {
           Ring& r = E4M3 ? rr : kr;
 #pragma unroll 1
           for (int i = 0; i * VR < keys; ++i) {
-            if (E4M3 && own) continue;
-            if (!warp_wait(E4M3 ? &r_empty[r.st] : &k_empty[r.st], r.ph ^ 1, a.err)) return false;
-            uint64_t* fb = E4M3 ? &r_full[r.st] : &k_full[r.st];
-            uint8_t* d = (E4M3 ? sRaw : sK) + r.st * SLOT;
-            constexpr int ROW = E4M3 ? 64 : 128;  // bytes of a row in one column block
-            if (own) {
-              if (lane == 0) sm100::mbar_expect_tx(fb, DA * min(a.T, VK) * 128);
-              __syncwarp();
-              if (lane < DA) sm100::tma_load_4d(d + lane * (VK * 128), &tv, fb, 64 * lane, p.hk, i * VK, p.s);
-            } else {
-              const int runs = (min(VR, keys - i * VR) + vb - 1) / vb;
-              if (lane == 0) sm100::mbar_expect_tx(fb, VA * runs * vb * ROW);
-              __syncwarp();
+            ok = ok && wait(E4M3 ? &r_empty[r.st] : &k_empty[r.st], r.ph ^ 1, a.err);
+            if (sm100::elect_one() && ok) {
+              uint64_t* fb = E4M3 ? &r_full[r.st] : &k_full[r.st];
+              uint8_t* d = (E4M3 ? sRaw : sK) + r.st * SLOT;
+              if (own) {
+                sm100::mbar_expect_tx(fb, DA * min(a.T, VK) * 128);
 #pragma unroll
-              for (int x0 = 0; x0 < VA * (VR / 16); x0 += 32) {  // lanes over column blocks x runs
-                const int x = x0 + lane, j = x % VA, u = x / VA;
-                const int row = __shfl_sync(0xffffffff, rows, (i * VR + u * vb) / 16 & 7);
-                if (u < runs)
-                  sm100::tma_load_2d(d + j * (VR * ROW) + u * vb * ROW, &tvp, fb, 64 * j, row);
+                for (int j = 0; j < DA; ++j)
+                  sm100::tma_load_4d(d + j * (VK * 128), &tv, fb, 64 * j, p.hk, i * VK, p.s);
+              } else {
+                const int runs = (min(VR, keys - i * VR) + vb - 1) / vb;
+                sm100::mbar_expect_tx(fb, VA * runs * vb * ROW);
+                for (int u = 0; u < runs; ++u) {
+                  const int row = rows[(i * VR + u * vb) / 16];
+#pragma unroll
+                  for (int j = 0; j < VA; ++j)
+                    sm100::tma_load_2d(d + j * (VR * ROW) + u * vb * ROW, &tvp, fb, 64 * j, row);
+                }
               }
             }
             __syncwarp();
             r.step(E4M3 ? NR : NK);
           }
         }
-        return true;
       });
     }
     // drain: every issued copy has landed before the CTA may exit
-    if (!E4M3 && pc > 0) warp_wait(q_full, (pc - 1) & 1, a.err);
+    if (!E4M3 && pc > 0) wait(q_full, (pc - 1) & 1, a.err);
     for (int i = 0; i < NK; ++i) {  // slots that were never armed count as empty
-      warp_wait(&k_empty[kr.st], kr.ph ^ 1, a.err);
+      wait(&k_empty[kr.st], kr.ph ^ 1, a.err);
       kr.step(NK);
     }
     for (int i = 0; i < NR; ++i) {
-      warp_wait(&r_empty[rr.st], rr.ph ^ 1, a.err);
+      wait(&r_empty[rr.st], rr.ph ^ 1, a.err);
       rr.step(NR);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
+    // The tensor cores wait for this warp's own instructions first, so the loops hold little but
+    // waits (the whole warp) and products (one elected lane: ptxas then keeps the operands
+    // uniform, without a loop over lanes around each); descriptors are a constant plus offsets
+    // in 16-byte units.
     constexpr uint32_t idesc_o = E4M3 ? sm100::idesc_f16(BM, DT, false, true) : sm100::idesc_bf16(BM, DT, false, true);
-    const uint32_t q_base = sm100::smem_u32(sQ);
+    const uint64_t dq = sm100::smem_desc_sw128(sm100::smem_u32(sQ), 0, 1024);
+    const uint64_t dk = sm100::smem_desc_sw128(sm100::smem_u32(sK), 0, 1024);
+    const uint64_t dv = sm100::smem_desc_sw128(sm100::smem_u32(sV), VK * 128, 1024);
     Ring kr, vr;
     int n = 0, ns = 0, pc = 0;  // PV tile, S tile, piece
     bool ok = true;
-    while (ok && walk.next(a, p)) {
-      ok = warp_wait(q_full, pc & 1, a.err);
-      ok = ok && product_order(p.t0, p.t1, [&](int t, bool pv) -> bool {
+    while (walk.next(a, p)) {
+      ok = ok && wait(q_full, pc & 1, a.err);
+      product_order(p.t0, p.t1, [&](int t, bool pv) {
         const int keys = p.keys(t);
         const bool own = t == p.nt;
         if (!pv) {
-          // the buffer's last reader, and every product before it, is done
-          if (n > 0 && !warp_wait(o_done, (n - 1) & 1, a.err)) return false;
           const uint32_t cols = max(16, (keys + 15) & ~15);
           const uint32_t idesc = sm100::idesc_bf16(BM, 16, false, false) - (2u << 17) + ((cols >> 3) << 17);
           const uint32_t idesc8 = idesc & ~((1u << 7) | (1u << 10));  // e4m3 x e4m3; bits 7 / 10: e5m2
           const uint32_t d = tmem + C::S_COL + (ns & 1) * BN;
-          if constexpr (E4M3) {
-            if (own) {  // (Q hi + Q lo) (K hi + K lo), the two K matrices of 64 rows one after the other
-              const uint32_t k_at[2] = {sm100::smem_u32(sK + kr.st * SLOT),
-                                        sm100::smem_u32(sK + (DT == 256 ? (kr.st + 1) % NK : kr.st) * SLOT) +
-                                            (DT == 256 ? 0 : MAX_NODES * 128)};
-              for (int j = 0; j < KS; ++j) {
-                if (!warp_wait(&k_full[kr.st], kr.ph, a.err)) return false;
-                kr.step(NK);
-              }
-              sm100::tc_fence_after();
-              if (lane == 0) {
-                for (int x = 0; x < 4; ++x)
-                  for (int kk = 0; kk < DT / 32; ++kk) {
-                    const uint32_t off = (kk & 3) * 32, at = kk >> 2;
-                    sm100::mma_f8(d, sm100::smem_desc_sw128(q_base + (x & 1) * (BM * DT) + at * (BM * 128) + off, 0, 1024),
-                           sm100::smem_desc_sw128(k_at[x >> 1] + at * (MAX_NODES * 128) + off, 0, 1024),
-                           idesc8 | (x & 1) << 7 | (x >> 1) << 10,
-                           x + kk > 0 ? 1u : 0u);
-                  }
-                for (int j = 0; j < KS; ++j) sm100::mma_commit(&k_empty[(kr.st + NK - 1 - j) % NK]);
-              }
-              __syncwarp();
-            }
-          }
-          if (!E4M3 || !own) {
-#pragma unroll 1
+          // the buffer's last reader, and every product before it, is done
+          if (n > 0) ok = ok && wait(o_done, (n - 1) & 1, a.err);
+          if (E4M3 && own) {  // (Q hi + Q lo) (K hi + K lo), the two K matrices of 64 rows one after the other
+            const Ring k0 = kr;
             for (int j = 0; j < KS; ++j) {
-              if (!warp_wait(&k_full[kr.st], kr.ph, a.err)) return false;
+              ok = ok && wait(&k_full[kr.st], kr.ph, a.err);
+              kr.step(NK);
+            }
+            sm100::tc_fence_after();
+            if (sm100::elect_one() && ok) {
+              const uint64_t hi = dk + k0.st * (SLOT / 16);
+              const uint64_t lo = DT == 256 ? dk + (k0.st + 1) % NK * (SLOT / 16) : hi + MAX_NODES * 8;
+#pragma unroll 1
+              for (int x = 0; x < 4; ++x) {
+#pragma unroll
+                for (int kk = 0; kk < DT / 32; ++kk)
+                  sm100::mma_f8(d, dq + (x & 1) * (BM * DT / 16) + (kk >> 2) * (BM * 8) + (kk & 3) * 2,
+                                (x >> 1 ? lo : hi) + (kk >> 2) * (MAX_NODES * 8) + (kk & 3) * 2,
+                                idesc8 | (x & 1) << 7 | (x >> 1) << 10, x + kk > 0 ? 1u : 0u);
+              }
+              sm100::mma_commit(&k_empty[k0.st]);
+              if (KS == 2) sm100::mma_commit(&k_empty[(k0.st + 1) % NK]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+              ok = ok && wait(&k_full[kr.st], kr.ph, a.err);
               sm100::tc_fence_after();
-              if (lane == 0) {
-                const uint32_t base = sm100::smem_u32(sK + kr.st * SLOT);
+              if (sm100::elect_one() && ok) {
+                const uint64_t kd = dk + kr.st * (SLOT / 16);
                 if constexpr (E4M3) {
 #pragma unroll
                   for (int x = 0; x < 2; ++x)
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                      sm100::mma_f8(d, sm100::smem_desc_sw128(q_base + x * (BM * DT) + j * (BM * 128) + kk * 32, 0, 1024),
-                             sm100::smem_desc_sw128(base + kk * 32, 0, 1024), idesc8 | x << 7,
-                             j + x + kk > 0 ? 1u : 0u);
+                      sm100::mma_f8(d, dq + (x * (BM * DT / 16) + j * (BM * 8) + kk * 2), kd + kk * 2, idesc8 | x << 7,
+                                    j + x + kk > 0 ? 1u : 0u);
                 } else {
 #pragma unroll
                   for (int kk = 0; kk < 4; ++kk)
-                    sm100::mma_bf16(d, sm100::smem_desc_sw128(q_base + j * (BM * 128) + kk * 32, 0, 1024),
-                                    sm100::smem_desc_sw128(base + kk * 32, 0, 1024), idesc, j + kk > 0 ? 1u : 0u);
+                    sm100::mma_bf16(d, dq + (j * (BM * 8) + kk * 2), kd + kk * 2, idesc, j + kk > 0 ? 1u : 0u);
                 }
                 sm100::mma_commit(&k_empty[kr.st]);
+                if (j == KS - 1) sm100::mma_commit(&s_full[ns & 1]);
               }
-              __syncwarp();
               kr.step(NK);
             }
           }
-          if (lane == 0) {
-            sm100::mma_commit(&s_full[ns & 1]);
-            if (t == p.t1 - 1) sm100::mma_commit(q_empty);
+          if (((E4M3 && own) || (!E4M3 && t == p.t1 - 1)) && sm100::elect_one() && ok) {
+            if (E4M3 && own) sm100::mma_commit(&s_full[ns & 1]);
+            if (!E4M3) sm100::mma_commit(q_empty);
           }
-          __syncwarp();
           ++ns;
         } else {
           const int pb = n & 1;
-          bool have_p = false;
+          const uint32_t ps = tmem + C::S_COL + pb * BN;
+          Ring& r = E4M3 ? vr : kr;
+          ok = ok && wait(&p_full[pb], (n >> 1) & 1, a.err);
+          if (t == p.t0 && pc > 0) ok = ok && wait(o_free, (pc - 1) & 1, a.err);
+          auto product = [&](int k16, uint64_t bd) {  // P of 16 keys: 8 columns of its half's 64
+#pragma unroll
+            for (int x = 0; x < C::PP; ++x)
+              sm100::mma_f16_ts(tmem, ps + (k16 >> 2) * 64 + x * 32 + (k16 & 3) * 8, bd, idesc_o,
+                                (t > p.t0 || k16 + x > 0) ? 1u : 0u);
+          };
+          if (keys == BN) {
+#pragma unroll
+            for (int i = 0; i < DA; ++i) {
+              ok = ok && wait(&v_full[r.st], r.ph, a.err);
+              sm100::tc_fence_after();
+              if (sm100::elect_one() && ok) {
+#pragma unroll
+                for (int kk = 0; kk < VK / 16; ++kk)
+                  product(i * (VK / 16) + kk, dv + r.st * (SLOT / 16) + kk * 128);
+                sm100::mma_commit(&v_empty[r.st]);
+                if (i == DA - 1) sm100::mma_commit(o_done);
+              }
+              r.step(E4M3 ? NV : NK);
+            }
+          } else {
 #pragma unroll 1
-          for (int i = 0; i * VK < keys; ++i) {
-            Ring& r = E4M3 ? vr : kr;
-            if (!warp_wait(&v_full[r.st], r.ph, a.err)) return false;
-            uint8_t* tile = sV + r.st * SLOT;
-            const int live = min(VK, keys - i * VK);
-            if constexpr (!E4M3) {  // rows of V beyond the end, up to the next product's edge
-              if (live & 15) {
-                const int dead = 16 - (live & 15);
-                for (int x = lane; x < dead * 8 * DA; x += 32)
-                  *reinterpret_cast<uint4*>(tile + tile_offset(VK, live + x / (8 * DA), x % (8 * DA))) =
+            for (int i = 0; i * VK < keys; ++i) {
+              const int live = min(VK, keys - i * VK);
+              ok = ok && wait(&v_full[r.st], r.ph, a.err);
+              if (!E4M3 && (live & 15)) {  // rows beyond the end, up to the next product's edge
+                for (int x = lane; x < (16 - (live & 15)) * 8 * DA; x += 32)
+                  *reinterpret_cast<uint4*>(sV + r.st * SLOT + tile_offset(VK, live + x / (8 * DA), x % (8 * DA))) =
                       make_uint4(0, 0, 0, 0);
                 sm100::fence_proxy_async_smem();
                 __syncwarp();
               }
-            }
-            if (!have_p) {
-              if (!warp_wait(&p_full[pb], (n >> 1) & 1, a.err)) return false;
-              if (t == p.t0 && pc > 0 && !warp_wait(o_free, (pc - 1) & 1, a.err)) return false;
-              have_p = true;
-            }
-            sm100::tc_fence_after();
-            if (lane == 0) {
-              const uint32_t base = sm100::smem_u32(tile), ps = tmem + C::S_COL + pb * BN;
-              for (int kk = 0; kk * 16 < live; ++kk) {
-                const int k16 = i * (VK / 16) + kk;  // P of 16 keys: 8 columns of its half's 64
-                const uint64_t bd = sm100::smem_desc_sw128(base + kk * 2048, VK * 128, 1024);
-#pragma unroll
-                for (int x = 0; x < C::PP; ++x)
-                  sm100::mma_f16_ts(tmem, ps + (k16 >> 2) * 64 + x * 32 + (k16 & 3) * 8, bd, idesc_o,
-                                    (t > p.t0 || k16 + x > 0) ? 1u : 0u);
+              sm100::tc_fence_after();
+              if (sm100::elect_one() && ok) {
+#pragma unroll 1
+                for (int kk = 0; kk * 16 < live; ++kk)
+                  product(i * (VK / 16) + kk, dv + r.st * (SLOT / 16) + kk * 128);
+                sm100::mma_commit(&v_empty[r.st]);
               }
-              sm100::mma_commit(&v_empty[r.st]);
+              r.step(E4M3 ? NV : NK);
             }
-            __syncwarp();
-            r.step(E4M3 ? NV : NK);
+            if (sm100::elect_one() && ok) sm100::mma_commit(o_done);
           }
-          if (!have_p) {  // no keys at all: O is not read
-            if (!warp_wait(&p_full[pb], (n >> 1) & 1, a.err)) return false;
-            if (t == p.t0 && pc > 0 && !warp_wait(o_free, (pc - 1) & 1, a.err)) return false;
-          }
-          if (lane == 0) {
-            sm100::mma_commit(o_done);
-            if (t == p.t1 - 1) sm100::mma_commit(o_last);
-          }
-          __syncwarp();
+          if (t == p.t1 - 1 && sm100::elect_one() && ok) sm100::mma_commit(o_last);
           ++n;
         }
-        return true;
       });
       ++pc;
     }
   } else if (warp < 2 + SOFT_WARPS) {
     // ---------------------------------------------------------- softmax warps
     // Two threads per row, each with 64 of a tile's 128 scores and half of O's columns. They
-    // exchange their maxima through shared memory. No early exit: a warp whose wait ran out
-    // (ok = false) keeps meeting its partner at the barriers, only without further waits.
+    // exchange their maxima through shared memory.
     const int qw = warp & 3, half = (warp - 2) >> 2;  // TMEM lane quarter, column half
     const int row = qw * 32 + lane;
     const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
@@ -648,7 +644,10 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
     const bool warp_on = qw * 32 < rows;
     int n = 0, pc = 0;
     bool ok = true;
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) { ok = ok && warp_wait(bar, parity, a.err); };
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+      if (lane == 0) ok = ok && wait(bar, parity, a.err);
+      __syncwarp();
+    };
     auto exchange = [&](float* buf, float v) -> float {  // the partner's value
       buf[half * BM + row] = v;
       sm100::named_sync(1 + qw, 64);
@@ -894,8 +893,12 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
       if (lane * 8 < a.D) w = *reinterpret_cast<const uint4*>(x + lane * 8);
       return row_exponent(__reduce_max_sync(0xffffffff, finite_top(w)), at);
     };
-    while (ok && walk.next(a, p)) {
-      ok = product_order(p.t0, p.t1, [&](int t, bool pv) -> bool {
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+      if (lane == 0) ok = ok && wait(bar, parity, a.err);
+      __syncwarp();
+    };
+    while (walk.next(a, p)) {
+      product_order(p.t0, p.t1, [&](int t, bool pv) {
         const int keys = p.keys(t);
         const bool own = t == p.nt;
         const bf16* nv = a.v + p.s * a.v_bs + p.hk * a.v_hs;
@@ -904,7 +907,7 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
           if (own) {
             const Ring k0 = kr;
             for (int j = 0; j < KS; ++j) {
-              if (!warp_wait(&k_empty[kr.st], kr.ph ^ 1, a.err)) return false;
+              wait_all(&k_empty[kr.st], kr.ph ^ 1);
               kr.step(NK);
             }
             uint8_t* hi_at = sK + k0.st * SLOT;
@@ -952,7 +955,7 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
           } else {
             for (int j = 0; j < KS; ++j) kr.step(NK);
             if (cw == n % CONV_WARPS) {
-              if (!warp_wait(&e_full[fb], (n / FAC) & 1, a.err)) return false;
+              wait_all(&e_full[fb], (n / FAC) & 1);
               const uint8_t* ex = sExp + fb * 2 * BN;
               int e[4], top = EXP_MIN;
 #pragma unroll
@@ -974,7 +977,7 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
           ++n;
         } else if (own) {
           for (int i = 0; i * VK < keys; ++i) {
-            if (!warp_wait(&v_empty[vr.st], vr.ph ^ 1, a.err)) return false;
+            wait_all(&v_empty[vr.st], vr.ph ^ 1);
             uint8_t* tile = sV + vr.st * SLOT;
             for (int r = cw; r < min(VK, (keys - i * VK + 15) & ~15); r += CONV_WARPS) {
               uint4 w = make_uint4(0, 0, 0, 0);
@@ -993,8 +996,8 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
           const int r8 = lane >> 2, q4 = lane & 3;  // row of 8, 16 codes of 64
           for (int i = 0; i * VK < keys; ++i) {
             constexpr int PER = C::RK / VK;  // f16 slots that one slot of codes fills
-            if (i % PER == 0 && !warp_wait(&r_full[rr.st], rr.ph, a.err)) return false;
-            if (!warp_wait(&v_empty[vr.st], vr.ph ^ 1, a.err)) return false;
+            if (i % PER == 0) wait_all(&r_full[rr.st], rr.ph);
+            wait_all(&v_empty[vr.st], vr.ph ^ 1);
             const uint8_t* raw = sRaw + rr.st * SLOT + (i % PER) * VK * 64;
             uint8_t* tile = sV + vr.st * SLOT;
 #pragma unroll 4
@@ -1028,7 +1031,6 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
             vr.step(NV);
           }
         }
-        return true;
       });
     }
   }
@@ -1200,6 +1202,7 @@ std::vector<at::Tensor> tree_attention(at::Tensor q, at::Tensor k, at::Tensor v,
   a.table = table.data_ptr<int>();
   a.pages = c.pages, a.max_pages = table.size(1);
   a.b = (int)b, a.T = (int)T, a.Hq = (int)Hq, a.Hk = c.heads, a.D = (int)D, a.page = c.page;
+  a.page_log2 = c.page == 16 ? 4 : c.page == 32 ? 5 : c.page == 64 ? 6 : 7;
   a.G = (int)Hq / c.heads;
   a.HB = (a.G + tattn::BM - 1) / tattn::BM;
   a.GT = (a.G + a.HB - 1) / a.HB;
