@@ -14,8 +14,17 @@
 // Products of decays (rather than e^{G_t - G_a} of summed logs) keep their relative
 // precision when fast and slow decays meet, and g = -inf (a reset) needs no care.
 //
-// First form: one CTA per (value head, sequence), thread = value channel with its column
-// of the state in registers; everything in fp32.
+// Bound: the states' bytes (4 D^2 per head and sequence, each read once, and written once where
+// it moves on); for wide trees and prompts the T x T algebra and the products with S.
+//
+// A CTA takes 64 value channels (columns of S are independent) of one head, a warp 16 of
+// them, as S^T in the accumulator layout of mma.sync m16n8k16 (fp32, 64 registers), which is
+// also the layout of its A operand: S^T K^T and S^T Q^T take S as the sum of three bf16
+// matrices (24 bits) against the raw bf16 keys, exact up to fp32 accumulation; the norms are
+// factored out. Moving S on adds U^T K, with U split the same way, into the same registers.
+// (mma.sync and not tcgen05: the fp32 state has to be split in registers anyway, and at the
+// sizes of a decoding step the loads of S dominate.) The unit triangular system in u is
+// solved by blocks of 16 nodes in fp32.
 #include "decode.h"
 #include "sm100.cuh"
 
@@ -43,18 +52,6 @@ struct Args {
   int* err;
 };
 
-__device__ __forceinline__ float block_sum(float x, float* buf) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffff, x, o);
-  const int nw = (blockDim.x + 31) / 32;
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = x;
-  __syncthreads();
-  float s = 0.f;
-  for (int i = 0; i < nw; ++i) s += buf[i];
-  return s;
-}
-
 // row of the state pool of sequence s, or -1 (idle or out of range)
 __device__ __forceinline__ int64_t state_row(const Args& a, int s) {
   const int64_t r = a.rows ? a.rows[s] : s;
@@ -74,154 +71,485 @@ __device__ __forceinline__ int node_count(const Args& a, int s) {
   return c;
 }
 
-// Threads: max(D, 32); threads at or beyond D take part in reductions only.
-template <int D>
-__global__ void __launch_bounds__(D < 32 ? 32 : D) gdn_advance_kernel(Args a) {
-  __shared__ float ks[D], qs[D], buf[8];
-  const int h = blockIdx.x, s = blockIdx.y, c = threadIdx.x, hk = h / a.groups;
-  const bool on = c < D;
-  const int64_t row = state_row(a, s);
-  const int cnt = row < 0 ? 0 : node_count(a, s);
-  float S[D];
-  const float* st = a.state + (row < 0 ? 0 : row) * a.s_rs + (int64_t)h * D * D;
-#pragma unroll
-  for (int i = 0; i < D; ++i) S[i] = on && row >= 0 ? st[i * D + c] : 0.f;
-  for (int t = 0; t < cnt; ++t) {
-    const float kv = on ? bf(a.k[s * a.k_bs + t * a.k_ts + hk * a.k_hs + c]) : 0.f;
-    const float qv = on ? bf(a.q[s * a.q_bs + t * a.q_ts + hk * a.q_hs + c]) : 0.f;
-    const float ik = rsqrtf(block_sum(kv * kv, buf) + 1e-6f);
-    const float iq = rsqrtf(block_sum(qv * qv, buf) + 1e-6f) * rsqrtf((float)D);
-    if (on) ks[c] = kv * ik, qs[c] = qv * iq;
-    __syncthreads();
-    const float eg = expf(a.g[s * a.g_bs + t * a.g_ts + h]);
-    const float be = bf(a.beta[s * a.b_bs + t * a.b_ts + h]);
-    float x = 0.f;
-#pragma unroll
-    for (int i = 0; i < D; ++i) {
-      S[i] *= eg;
-      x = fmaf(S[i], ks[i], x);
-    }
-    const float u = on ? be * (bf(a.v[s * a.v_bs + t * a.v_ts + h * a.v_hs + c]) - x) : 0.f;
-    float o = 0.f;
-#pragma unroll
-    for (int i = 0; i < D; ++i) {
-      S[i] = fmaf(ks[i], u, S[i]);
-      o = fmaf(S[i], qs[i], o);
-    }
-    if (on) a.out[(((int64_t)s * a.T + t) * a.nv + h) * D + c] = __float2bfloat16(o);
-  }
-  for (int t = cnt; t < a.T; ++t)
-    if (on) a.out[(((int64_t)s * a.T + t) * a.nv + h) * D + c] = __float2bfloat16(0.f);
-  if (row < 0 || !on) return;
-  float* so = a.out_state + row * a.o_rs + (int64_t)h * D * D;
-#pragma unroll
-  for (int i = 0; i < D; ++i) so[i * D + c] = S[i];
+// ------------------------------------------------------------------ tensor-core pieces
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int D>
-__global__ void __launch_bounds__(D < 32 ? 32 : D) gdn_verify_kernel(Args a) {
-  extern __shared__ float sm[];
-  float* ks = sm;                // [T][D] normalised keys
-  float* qs = ks + a.T * D;      // [T][D]
-  float* us = qs + a.T * D;      // [T][D]
-  float* dec = us + a.T * D;     // [T][T] decays between nodes
-  float* kk = dec + a.T * a.T;   // [T] products of the current node with every earlier key
-  float* qk = kk + a.T;          // [T]
-  float* w = qk + a.T;           // [T] decays from the carried state
-  __shared__ float buf[8];
-  const int h = blockIdx.x, s = blockIdx.y, c = threadIdx.x, hk = h / a.groups;
-  const bool on = c < D;
-  const int64_t row = state_row(a, s);
-  const int cnt = row < 0 ? 0 : node_count(a, s);
-  float S[D];
-  const float* st = a.state + (row < 0 ? 0 : row) * a.s_rs + (int64_t)h * D * D;
-#pragma unroll
-  for (int i = 0; i < D; ++i) S[i] = on && row >= 0 ? st[i * D + c] : 0.f;
-  for (int t = 0; t < cnt; ++t) {
-    const float kv = on ? bf(a.k[s * a.k_bs + t * a.k_ts + hk * a.k_hs + c]) : 0.f;
-    const float qv = on ? bf(a.q[s * a.q_bs + t * a.q_ts + hk * a.q_hs + c]) : 0.f;
-    const float ik = rsqrtf(block_sum(kv * kv, buf) + 1e-6f);
-    const float iq = rsqrtf(block_sum(qv * qv, buf) + 1e-6f) * rsqrtf((float)D);
-    if (on) ks[t * D + c] = kv * ik, qs[t * D + c] = qv * iq;
-    int p = a.parents[s * a.p_bs + t];
-    if (p < -1 || p >= t) {
-      if (c == 0) atomicExch(a.err, ERR_INDEX);
-      p = -1;
-    }
-    const float eg = expf(a.g[s * a.g_bs + t * a.g_ts + h]);
-    const float be = bf(a.beta[s * a.b_bs + t * a.b_ts + h]);
-    for (int j = c; j <= t; j += blockDim.x)  // row p holds columns up to p
-      dec[t * a.T + j] = j == t ? 1.f : j > p ? 0.f : eg * dec[p * a.T + j];
-    if (c == 0) w[t] = p < 0 ? eg : eg * w[p];
-    __syncthreads();
-    for (int j = c; j <= t; j += blockDim.x) {
-      float x = 0.f, y = 0.f;
-      for (int i = 0; i < D; ++i) {
-        x = fmaf(ks[t * D + i], ks[j * D + i], x);
-        y = fmaf(qs[t * D + i], ks[j * D + i], y);
-      }
-      kk[j] = x * dec[t * a.T + j];
-      qk[j] = y * dec[t * a.T + j];
-    }
-    __syncthreads();
-    float x = 0.f, y = 0.f;
-#pragma unroll
-    for (int i = 0; i < D; ++i) {
-      x = fmaf(S[i], ks[t * D + i], x);
-      y = fmaf(S[i], qs[t * D + i], y);
-    }
-    x *= w[t], y *= w[t];
-    if (on) {
-      for (int j = 0; j < t; ++j) {
-        x = fmaf(kk[j], us[j * D + c], x);
-        y = fmaf(qk[j], us[j * D + c], y);
-      }
-      const float u = be * (bf(a.v[s * a.v_bs + t * a.v_ts + h * a.v_hs + c]) - x);
-      us[t * D + c] = u;
-      const int64_t at = (((int64_t)s * a.T + t) * a.nv + h) * D + c;
-      a.u[at] = u;
-      a.out[at] = __float2bfloat16(fmaf(qk[t], u, y));
-    }
-  }
-  for (int t = cnt; t < a.T; ++t)
-    if (on) {
-      const int64_t at = (((int64_t)s * a.T + t) * a.nv + h) * D + c;
-      a.u[at] = 0.f;
-      a.out[at] = __float2bfloat16(0.f);
-    }
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(sm100::smem_u32(p)));
 }
 
+// x = hi + mid + lo in bf16, for a pair of values; the parts packed
+__device__ __forceinline__ void split3(float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  const float2 hf = __bfloat1622float2(h);
+  const float rx = x - hf.x, ry = y - hf.y;
+  const __nv_bfloat162 m = __floats2bfloat162_rn(rx, ry);
+  const float2 mf = __bfloat1622float2(m);
+  const __nv_bfloat162 l = __floats2bfloat162_rn(rx - mf.x, ry - mf.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  mid = *reinterpret_cast<const uint32_t*>(&m);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// One warp's 16 value channels of S^T: register [j][..] holds key channels 8j + 2q, + 1 of
+// value channels 2g (first two) and 2g + 1 (last two), lane = 4g + q.
 template <int D>
-__global__ void __launch_bounds__(D < 32 ? 32 : D) gdn_accept_kernel(Args a) {
-  __shared__ float ks[D], buf[8];
-  const int h = blockIdx.x, s = blockIdx.y, c = threadIdx.x, hk = h / a.groups;
-  const bool on = c < D;
+struct State {
+  float s[D / 8][4];
+  __device__ __forceinline__ void load(const float* p, int g, int q) {
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float2 x = *reinterpret_cast<const float2*>(p + (int64_t)(8 * j + 2 * q + i) * D + 2 * g);
+        s[j][i] = x.x;
+        s[j][2 + i] = x.y;
+      }
+  }
+  __device__ __forceinline__ void store(float* p, int g, int q) const {
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<float2*>(p + (int64_t)(8 * j + 2 * q + i) * D + 2 * g) = make_float2(s[j][i], s[j][2 + i]);
+  }
+  __device__ __forceinline__ void scale(float f) {
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[j][i] *= f;
+  }
+  // S^T += W^T K over 16 rows: w(row, value pair) in fp32, K rows bf16 in shared memory
+  template <int US, int KS>
+  __device__ __forceinline__ void add(const float* u, const float* coef, const bf16* k, int lane) {
+    const int g = lane >> 2, q = lane & 3;
+    uint32_t a[3][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = 8 * h + 2 * q;
+      const float2 x = *reinterpret_cast<const float2*>(u + r * US + 2 * g);
+      const float2 y = *reinterpret_cast<const float2*>(u + (r + 1) * US + 2 * g);
+      const float c0 = coef[r], c1 = coef[r + 1];
+      split3(x.x * c0, y.x * c1, a[0][2 * h], a[1][2 * h], a[2][2 * h]);
+      split3(x.y * c0, y.y * c1, a[0][2 * h + 1], a[1][2 * h + 1], a[2][2 * h + 1]);
+    }
+#pragma unroll
+    for (int j = 0; j < D / 8; j += 2) {
+      uint32_t b[4];  // rows 0-7 and 8-15 of key channels 8j.., then of 8j + 8..
+      ldsm_x4_trans(b, k + ((lane & 7) + (lane & 8)) * KS + 8 * j + (lane >> 4) * 8);
+#pragma unroll
+      for (int x = 0; x < 3; ++x) {
+        mma16816(s[j], a[x], b[0], b[1]);
+        mma16816(s[j + 1], a[x], b[2], b[3]);
+      }
+    }
+  }
+};
+
+// 16-byte chunks of rows [0, rows) of D channels into shared memory (zeros at and beyond
+// `live`) and 1 / sqrt(|row|^2 + 1e-6) of each.
+template <int D, int ST>
+__device__ __forceinline__ void load_rows(const bf16* src, int64_t ts, int live, int rows, bf16* dst, float* inv) {
+  constexpr int L = D / 8;  // lanes of one row
+  for (int i = threadIdx.x; i < (rows * L + 31) / 32 * 32; i += blockDim.x) {
+    const int r = i / L, c = i % L;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (r < live) w = *reinterpret_cast<const uint4*>(src + r * ts + c * 8);
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = __uint_as_float(in[e] << 16), y = __uint_as_float(in[e] & 0xffff0000u);
+      ss = fmaf(x, x, fmaf(y, y, ss));
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffff, ss, o);
+    if (r < rows) {
+      *reinterpret_cast<uint4*>(dst + r * ST + c * 8) = w;
+      if (c == 0) inv[r] = rsqrtf(ss + 1e-6f);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ nodes (a tree, or tokens in chunks)
+template <int D, int NT>
+struct Nodes {
+  static constexpr int COLS = D < 64 ? D : 64;         // value channels of a CTA
+  static constexpr int THREADS = COLS * 2;             // a warp per 16
+  static constexpr int TP = NT < 2 ? 16 : 8 * NT;      // nodes held (zero padded)
+  static constexpr int KST = D + 8;                    // row strides: 4 banks apart
+  static constexpr int US = COLS + 4;
+  static constexpr int MS = TP + 4;
+  static constexpr int ROWS = TP * KST * 2;            // bytes of K or Q
+  static constexpr int YB = TP * US * 4;               // bytes of U or Y
+  static constexpr int QY = ROWS > YB ? ROWS : YB;     // Q, then Y
+  static constexpr int SMEM = ROWS + QY + YB + 2 * TP * MS * 4 + 8 * TP * 4;
+  static constexpr int BLK = TP < 16 ? TP : 16;
+};
+
+// TREE: T <= 8 NT nodes with parents; the state is only read. Otherwise tokens in chunks of
+// 8 NT whose state moves on.
+template <int D, int NT, bool TREE>
+__global__ void __launch_bounds__(Nodes<D, NT>::THREADS, 3) gdn_nodes_kernel(Args a) {
+  using C = Nodes<D, NT>;
+  constexpr int TP = C::TP, TN = 8 * NT, KST = C::KST, US = C::US, MS = C::MS, COLS = C::COLS, SL = D / COLS;
+  extern __shared__ __align__(16) uint8_t sm[];
+  bf16* ks = reinterpret_cast<bf16*>(sm);               // [TP][KST]
+  bf16* qs = reinterpret_cast<bf16*>(sm + C::ROWS);     // [TP][KST]
+  float* ys = reinterpret_cast<float*>(sm + C::ROWS);   // [TP][US], once Q is consumed
+  float* us = reinterpret_cast<float*>(sm + C::ROWS + C::QY);  // [TP][US] right-hand sides, then u
+  float* mt = us + TP * US;                             // [a][t] decays D[t, a], then M
+  float* at = mt + TP * MS;                             // [a][t] A
+  float* ik = at + TP * MS;                             // [TP] 1 / |k|
+  float* iq = ik + TP;                                  // [TP] D^-1/2 / |q|
+  float* eg = iq + TP;                                  // [TP] e^g
+  float* be = eg + TP;                                  // [TP] beta
+  float* wt = be + TP;                                  // [TP] decay from the carried state
+  float* cf = wt + TP;                                  // [TP] what u adds to the state
+  int* par = reinterpret_cast<int*>(cf + TP);           // [TP]
+  const int h = blockIdx.x / SL, cs = blockIdx.x % SL * COLS, s = blockIdx.y, hk = h / a.groups;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const int64_t row = state_row(a, s);
+  const int cnt = row < 0 ? 0 : node_count(a, s);
+  const int col0 = cs + 16 * warp;  // this warp's value channels
+  State<D> S;
+  if (row >= 0)
+    S.load(a.state + row * a.s_rs + (int64_t)h * D * D + col0, g, q);
+  else
+    S.scale(0.f);
+  const int64_t ob = ((int64_t)s * a.T * a.nv + h) * D + cs;  // outputs: node t at ob + t nv D
+  const int64_t ots = (int64_t)a.nv * D;
+
+  for (int t0 = 0; t0 < cnt; t0 += TN) {
+    const int n = min(cnt - t0, TN);
+    const bf16* kp = a.k + s * a.k_bs + t0 * a.k_ts + hk * a.k_hs;
+    const bf16* qp = a.q + s * a.q_bs + t0 * a.q_ts + hk * a.q_hs;
+    const bf16* vp = a.v + s * a.v_bs + t0 * a.v_ts + h * a.v_hs + col0 + 2 * g;
+    // v of this thread's accumulators, early
+    uint32_t v[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int t = 8 * j + 2 * q + i;
+        v[j][i] = t < n ? *reinterpret_cast<const uint32_t*>(vp + t * a.v_ts) : 0u;
+      }
+    if (t0 > 0) __syncthreads();  // the previous chunk's readers
+    load_rows<D, KST>(kp, a.k_ts, n, TP, ks, ik);
+    load_rows<D, KST>(qp, a.q_ts, n, TP, qs, iq);
+    for (int t = tid; t < TP; t += C::THREADS) {
+      const bool in = t < n;
+      eg[t] = in ? expf(a.g[s * a.g_bs + (t0 + t) * a.g_ts + h]) : 1.f;
+      be[t] = in ? bf(a.beta[s * a.b_bs + (t0 + t) * a.b_ts + h]) : 0.f;
+      if constexpr (TREE) {
+        int p = in ? a.parents[s * a.p_bs + t] : -1;
+        if (p < -1 || p >= t) {
+          atomicExch(a.err, ERR_INDEX);
+          p = -1;
+        }
+        par[t] = p;
+      }
+    }
+    for (int i = tid; i < TP * MS / 4; i += C::THREADS) reinterpret_cast<float4*>(mt)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (TN < TP)  // rows of u that no node fills
+      for (int i = tid; i < (TP - TN) * US; i += C::THREADS) us[TN * US + i] = 0.f;
+    __syncthreads();
+    // decays: a tree's rows walk up to the root, a chain's columns run down
+    if constexpr (TREE) {
+      for (int t = tid; t < TP; t += C::THREADS) {
+        float d = 1.f;
+        for (int i = t; i >= 0; i = par[i]) {
+          mt[i * MS + t] = d;
+          d *= eg[i];
+        }
+        wt[t] = d;
+      }
+    } else {
+      for (int i = tid; i <= TP; i += C::THREADS) {  // thread TP: from the carried state
+        float d = 1.f;
+#pragma unroll 8
+        for (int t = 0; t < TP; ++t) {
+          if (i == TP) {
+            d *= eg[t];
+            wt[t] = d;
+          } else if (t >= i) {
+            if (t > i) d *= eg[t];
+            mt[i * MS + t] = d;
+          }
+        }
+      }
+    }
+    // (S^T K^T), (S^T Q^T): value channels x nodes
+    float ka[NT][4], qa[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ka[j][i] = qa[j][i] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      uint32_t f[3][4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          split3(S.s[2 * kk + x][2 * y], S.s[2 * kk + x][2 * y + 1], f[0][2 * x + y], f[1][2 * x + y], f[2][2 * x + y]);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const bf16* kr = ks + (8 * j + g) * KST + 16 * kk + 2 * q;
+        const bf16* qr = qs + (8 * j + g) * KST + 16 * kk + 2 * q;
+        const uint32_t k0 = *reinterpret_cast<const uint32_t*>(kr), k1 = *reinterpret_cast<const uint32_t*>(kr + 8);
+        const uint32_t q0 = *reinterpret_cast<const uint32_t*>(qr), q1 = *reinterpret_cast<const uint32_t*>(qr + 8);
+#pragma unroll
+        for (int x = 2; x >= 0; --x) {
+          mma16816(ka[j], f[x], k0, k1);
+          mma16816(qa[j], f[x], q0, q1);
+        }
+      }
+    }
+    __syncthreads();  // decays are complete
+    if (!TREE && tid < TP) cf[tid] = ik[tid] * mt[tid * MS + TP - 1];
+    // right-hand sides beta (v - w S^T k^)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int t = 8 * j + 2 * q + i;
+        const float w = wt[t] * ik[t], b = be[t];
+        *reinterpret_cast<float2*>(us + t * US + 16 * warp + 2 * g) =
+            make_float2(b * (__uint_as_float(v[j][i] << 16) - w * ka[j][i]),
+                        b * (__uint_as_float(v[j][i] & 0xffff0000u) - w * ka[j][2 + i]));
+      }
+    if (!TREE) __syncthreads();  // cf before mt changes
+    // K K^T and Q K^T on the lower triangle, with their decays: M and A, transposed
+    const float rd = rsqrtf((float)D);
+    for (int mi = warp; mi < TP / 16; mi += C::THREADS / 32) {
+      for (int nj = 0; nj <= 2 * mi + 1; ++nj) {
+        float kk4[4] = {}, qk4[4] = {};
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const bf16* ar = ks + (16 * mi + g) * KST + 16 * kk + 2 * q;
+          const bf16* aq = qs + (16 * mi + g) * KST + 16 * kk + 2 * q;
+          const bf16* br = ks + (8 * nj + g) * KST + 16 * kk + 2 * q;
+          auto u32 = [](const bf16* p) { return *reinterpret_cast<const uint32_t*>(p); };
+          const uint32_t b0 = u32(br), b1 = u32(br + 8);
+          const uint32_t fa[4] = {u32(ar), u32(ar + 8 * KST), u32(ar + 8), u32(ar + 8 * KST + 8)};
+          const uint32_t fq[4] = {u32(aq), u32(aq + 8 * KST), u32(aq + 8), u32(aq + 8 * KST + 8)};
+          mma16816(kk4, fa, b0, b1);
+          mma16816(qk4, fq, b0, b1);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = 16 * mi + g + (i >> 1) * 8, c = 8 * nj + 2 * q + (i & 1);
+          const float d = mt[c * MS + t] * ik[c];
+          at[c * MS + t] = d * iq[t] * rd * qk4[i];
+          mt[c * MS + t] = c < t ? d * ik[t] * be[t] * kk4[i] : 0.f;
+        }
+      }
+    }
+    __syncthreads();
+    // Q is consumed: its place takes w S^T q^
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int t = 8 * j + 2 * q + i;
+        const float w = wt[t] * iq[t] * rd;
+        *reinterpret_cast<float2*>(ys + t * US + 16 * warp + 2 * g) = make_float2(w * qa[j][i], w * qa[j][2 + i]);
+      }
+    // (I + M) u = right-hand side, by blocks of 16 nodes; thread = (value channel, half of the rows)
+    const int c = tid % COLS, half = tid / COLS;
+    constexpr int R = TN < 16 ? TN / 2 : 8;  // rows of one thread
+    for (int r0 = 0; r0 < TN; r0 += 2 * R) {
+      if (r0 > 0) {
+        float x[R];
+        const int r = r0 + half * R;
+#pragma unroll
+        for (int i = 0; i < R; ++i) x[i] = us[(r + i) * US + c];
+#pragma unroll 4
+        for (int m = 0; m < r0; ++m) {
+          const float u = us[m * US + c];
+#pragma unroll
+          for (int i = 0; i < R; i += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(mt + m * MS + r + i);
+            x[i] -= f.x * u, x[i + 1] -= f.y * u, x[i + 2] -= f.z * u, x[i + 3] -= f.w * u;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) us[(r + i) * US + c] = x[i];
+        __syncthreads();
+      }
+      if (half == 0) {
+        float x[2 * R];
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i) x[i] = us[(r0 + i) * US + c];
+#pragma unroll
+        for (int m = 0; m + 1 < 2 * R; ++m)
+#pragma unroll
+          for (int i = (m + 1) & ~3; i < 2 * R; i += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(mt + (r0 + m) * MS + r0 + i);
+            if (i > m) x[i] -= f.x * x[m];
+            if (i + 1 > m) x[i + 1] -= f.y * x[m];
+            if (i + 2 > m) x[i + 2] -= f.z * x[m];
+            x[i + 3] -= f.w * x[m];
+          }
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i) us[(r0 + i) * US + c] = x[i];
+      }
+      __syncthreads();
+    }
+    // o = w S^T q^ + A u
+    for (int r = half * R; r < TN; r += 2 * R) {
+      if (r >= n) break;
+      float x[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) x[i] = ys[(r + i) * US + c];
+#pragma unroll 4
+      for (int m = 0; m < r + R; ++m) {
+        const float u = us[m * US + c];
+#pragma unroll
+        for (int i = 0; i < R; i += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(at + m * MS + r + i);
+          x[i] = fmaf(f.x, u, x[i]), x[i + 1] = fmaf(f.y, u, x[i + 1]);
+          x[i + 2] = fmaf(f.z, u, x[i + 2]), x[i + 3] = fmaf(f.w, u, x[i + 3]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (r + i < n) {
+          a.out[ob + (t0 + r + i) * ots + c] = __float2bfloat16(x[i]);
+          if constexpr (TREE) a.u[ob + (r + i) * ots + c] = us[(r + i) * US + c];
+        }
+    }
+    if constexpr (!TREE) {
+      S.scale(wt[TP - 1]);
+#pragma unroll 1
+      for (int r = 0; r < n; r += 16)
+        S.template add<US, KST>(us + r * US + 16 * warp, cf + r, ks + r * KST, lane);
+    }
+  }
+  for (int i = cnt * COLS + tid; i < a.T * COLS; i += C::THREADS) {  // padding
+    const int64_t o = ob + (i / COLS) * ots + i % COLS;
+    a.out[o] = __float2bfloat16(0.f);
+    if constexpr (TREE) a.u[o] = 0.f;
+  }
+  if (!TREE && row >= 0) S.store(a.out_state + row * a.o_rs + (int64_t)h * D * D + col0, g, q);
+}
+
+// ------------------------------------------------------------------ accepted path
+// S' = gamma S + sum over the path of (decay after the node) k^ u^T.
+template <int D>
+__global__ void __launch_bounds__(Nodes<D, 2>::THREADS) gdn_accept_kernel(Args a) {
+  using C = Nodes<D, 2>;
+  constexpr int KST = C::KST, US = C::US, COLS = C::COLS, SL = D / COLS;
+  __shared__ __align__(16) bf16 ks[16 * KST];
+  __shared__ __align__(16) float us[16 * US];
+  __shared__ float ik[16], cf[MAX_NODES];
+  __shared__ int node[MAX_NODES], count;
+  __shared__ float gamma;
+  const int h = blockIdx.x / SL, cs = blockIdx.x % SL * COLS, s = blockIdx.y, hk = h / a.groups;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int64_t row = state_row(a, s);
   if (row < 0) return;
-  float S[D];
-  const float* st = a.state + row * a.s_rs + (int64_t)h * D * D;
-#pragma unroll
-  for (int i = 0; i < D; ++i) S[i] = on ? st[i * D + c] : 0.f;
-  for (int j = 0; j < a.m; ++j) {
-    const int t = a.path[(int64_t)s * a.m + j];
-    if (t < 0 || t >= a.T) {
-      if (t != -1 && c == 0) atomicExch(a.err, ERR_INDEX);
-      continue;
+  State<D> S;
+  S.load(a.state + row * a.s_rs + (int64_t)h * D * D + cs + 16 * warp, g, q);
+  if (warp == 0) {
+    // nodes of the path in order, then the decay after each, from the last one back
+    int m = 0;
+    for (int j0 = 0; j0 < a.m; j0 += 32) {
+      int t = j0 + lane < a.m ? a.path[(int64_t)s * a.m + j0 + lane] : -1;
+      if (t < -1 || t >= a.T) {
+        atomicExch(a.err, ERR_INDEX);
+        t = -1;
+      }
+      const uint32_t on = __ballot_sync(0xffffffff, t >= 0);
+      if (t >= 0) {
+        const int at = m + __popc(on & ((1u << lane) - 1));
+        node[at] = t;
+        cf[at] = expf(a.g[s * a.g_bs + t * a.g_ts + h]);
+      }
+      m += __popc(on);
     }
-    const float kv = on ? bf(a.k[s * a.k_bs + t * a.k_ts + hk * a.k_hs + c]) : 0.f;
-    const float ik = rsqrtf(block_sum(kv * kv, buf) + 1e-6f);
-    if (on) ks[c] = kv * ik;
-    __syncthreads();
-    const float eg = expf(a.g[s * a.g_bs + t * a.g_ts + h]);
-    const float u = on ? a.u_in[(((int64_t)s * a.T + t) * a.nv + h) * D + c] : 0.f;
-#pragma unroll
-    for (int i = 0; i < D; ++i) S[i] = fmaf(ks[i], u, S[i] * eg);
-    __syncthreads();
+    __syncwarp();
+    if (lane == 0) {
+      float d = 1.f;
+      for (int j = m - 1; j >= 0; --j) {
+        const float e = cf[j];
+        cf[j] = d;
+        d *= e;
+      }
+      gamma = d;
+      count = m;
+    }
   }
-  if (!on) return;
-  float* so = a.out_state + row * a.o_rs + (int64_t)h * D * D;
+  __syncthreads();
+  const int m = count;
+  S.scale(gamma);
+  for (int r0 = 0; r0 < m; r0 += 16) {
+    if (r0 > 0) __syncthreads();
+    constexpr int L = D / 8, LU = COLS / 4;
+    for (int i = tid; i < 16 * L; i += C::THREADS) {  // key rows and their norms (L lanes a row)
+      const int r = i / L, c = i % L;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (r0 + r < m)
+        w = *reinterpret_cast<const uint4*>(a.k + s * a.k_bs + node[r0 + r] * a.k_ts + hk * a.k_hs + c * 8);
+      const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+      float ss = 0.f;
 #pragma unroll
-  for (int i = 0; i < D; ++i) so[i * D + c] = S[i];
+      for (int e = 0; e < 4; ++e) {
+        const float x = __uint_as_float(in[e] << 16), y = __uint_as_float(in[e] & 0xffff0000u);
+        ss = fmaf(x, x, fmaf(y, y, ss));
+      }
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffff, ss, o);
+      *reinterpret_cast<uint4*>(ks + r * KST + c * 8) = w;
+      if (c == 0) ik[r] = rsqrtf(ss + 1e-6f);
+    }
+    __syncthreads();
+    for (int i = tid; i < 16 * LU; i += C::THREADS) {
+      const int r = i / LU, c = i % LU;
+      float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r0 + r < m) {
+        w = *reinterpret_cast<const float4*>(a.u_in + (((int64_t)s * a.T + node[r0 + r]) * a.nv + h) * D + cs + c * 4);
+        const float f = ik[r];
+        w = make_float4(w.x * f, w.y * f, w.z * f, w.w * f);
+      }
+      *reinterpret_cast<float4*>(us + r * US + c * 4) = w;
+    }
+    for (int r = m + tid; r < ((m + 15) & ~15); r += C::THREADS) cf[r] = 0.f;
+    __syncthreads();
+    S.template add<US, KST>(us + 16 * warp, cf + r0, ks, lane);
+  }
+  S.store(a.out_state + row * a.o_rs + (int64_t)h * D * D + cs + 16 * warp, g, q);
+}
+
+template <int D, int NT, bool TREE>
+void launch_nodes(const Args& a, int64_t b) {
+  using C = Nodes<D, NT>;
+  static std::atomic<unsigned long long> attr{0};
+  once_per_device(attr, [&] {
+    NS_CUDA(cudaFuncSetAttribute(gdn_nodes_kernel<D, NT, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+  });
+  gdn_nodes_kernel<D, NT, TREE><<<dim3((unsigned)(a.nv * (D / C::COLS)), (unsigned)b), C::THREADS, C::SMEM, stream()>>>(a);
+}
+
+// the fewest nodes per pass that hold T (chunks of 64 beyond)
+template <int D, bool TREE>
+void launch_for(const Args& a, int64_t b) {
+  if (a.T <= 8)
+    launch_nodes<D, 1, TREE>(a, b);
+  else if (a.T <= 16)
+    launch_nodes<D, 2, TREE>(a, b);
+  else if (a.T <= 32)
+    launch_nodes<D, 4, TREE>(a, b);
+  else
+    launch_nodes<D, 8, TREE>(a, b);
 }
 
 }  // namespace gdnd
@@ -310,8 +638,7 @@ at::Tensor gdn_advance(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor g, a
   at::Tensor out = at::empty({d.b, d.T, d.nv, d.D}, v.options());
   if (out.numel() == 0) return out;
   d.a.out = reinterpret_cast<bf16*>(out.data_ptr());
-  const dim3 grid((unsigned)d.nv, (unsigned)d.b);
-#define NS_X(DD) gdnd::gdn_advance_kernel<DD><<<grid, DD < 32 ? 32 : DD, 0, stream()>>>(d.a);
+#define NS_X(DD) gdnd::launch_for<DD, false>(d.a, d.b);
   NS_GDN_CASES(d.D, NS_X)
 #undef NS_X
   NS_CUDA(cudaGetLastError());
@@ -331,17 +658,7 @@ std::vector<at::Tensor> gdn_verify(at::Tensor q, at::Tensor k, at::Tensor v, at:
   if (out.numel() == 0) return {out, u};
   d.a.out = reinterpret_cast<bf16*>(out.data_ptr());
   d.a.u = u.data_ptr<float>();
-  const dim3 grid((unsigned)d.nv, (unsigned)d.b);
-  const int smem = (int)((3 * d.T * d.D + d.T * d.T + 3 * d.T) * 4);
-#define NS_X(DD)                                                                                       \
-  {                                                                                                    \
-    static std::atomic<unsigned long long> attr{0};                                                    \
-    once_per_device(attr, [&] {                                                                        \
-      NS_CUDA(cudaFuncSetAttribute(gdnd::gdn_verify_kernel<DD>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
-                                   (3 * MAX_NODES * DD + MAX_NODES * MAX_NODES + 3 * MAX_NODES) * 4)); \
-    });                                                                                                \
-    gdnd::gdn_verify_kernel<DD><<<grid, DD < 32 ? 32 : DD, smem, stream()>>>(d.a);                     \
-  }
+#define NS_X(DD) gdnd::launch_for<DD, true>(d.a, d.b);
   NS_GDN_CASES(d.D, NS_X)
 #undef NS_X
   NS_CUDA(cudaGetLastError());
@@ -365,6 +682,7 @@ void gdn_accept(at::Tensor k, at::Tensor g, at::Tensor u, at::Tensor path, at::T
   NS_VALUE(path.device() == d.dev && path.scalar_type() == at::kInt && path.dim() == 2 && path.size(0) == d.b &&
                path.is_contiguous(),
            "gated_delta_accept: path must be contiguous int32 [b, m]");
+  NS_VALUE(d.T <= MAX_NODES && path.size(1) <= MAX_NODES, "gated_delta_accept: at most 64 nodes, and path entries");
   NS_VALUE(d.b < 65536 && d.nv < 65536, "gated delta rule: too many sequences or heads");
   bind_state(d, state, rows, &out_state);
   if (d.b * d.nv == 0) return;
@@ -377,8 +695,10 @@ void gdn_accept(at::Tensor k, at::Tensor g, at::Tensor u, at::Tensor path, at::T
   d.a.path = path.data_ptr<int>();
   d.a.T = (int)d.T, d.a.m = (int)path.size(1), d.a.nv = (int)d.nv, d.a.groups = (int)groups;
   d.a.err = device_error_flag();
-  const dim3 grid((unsigned)d.nv, (unsigned)d.b);
-#define NS_X(DD) gdnd::gdn_accept_kernel<DD><<<grid, DD < 32 ? 32 : DD, 0, stream()>>>(d.a);
+#define NS_X(DD)                                                                                       \
+  gdnd::gdn_accept_kernel<DD>                                                                          \
+      <<<dim3((unsigned)(d.nv * (DD / gdnd::Nodes<DD, 2>::COLS)), (unsigned)d.b), gdnd::Nodes<DD, 2>::THREADS, 0, \
+         stream()>>>(d.a);
   NS_GDN_CASES(d.D, NS_X)
 #undef NS_X
   NS_CUDA(cudaGetLastError());

@@ -205,8 +205,8 @@ def gated_delta_verify(q, k, v, g, beta, state, parents, groups=1, counts=None, 
 
 
 def gated_delta_accept(k, g, u, path, state, groups=1, rows=None, out_state=None):
-    """Move ``state`` on along the accepted nodes ``path`` [b, m] of a verified tree (root
-    first, -1 entries skipped): S <- e^{g_a} S + k_a u_a^T. k and g as given to
+    """Move ``state`` on along the accepted nodes ``path`` [b, m <= 64] of a verified tree
+    (root first, -1 entries skipped): S <- e^{g_a} S + k_a u_a^T. k and g as given to
     ``gated_delta_verify``, u as it returned it. In place unless ``out_state`` is given;
     returns the new states."""
     out_state = state if out_state is None else out_state
@@ -219,6 +219,7 @@ def gated_delta_accept(k, g, u, path, state, groups=1, rows=None, out_state=None
     _need(g.shape == (b, t, nv), "gated_delta_accept: g must be [b, T, nv]")
     _need(path.dim() == 2 and path.shape[0] == b and path.dtype == torch.int32,
           "gated_delta_accept: path must be int32 [b, m]")
+    _need(t <= MAX_NODES and path.shape[1] <= MAX_NODES, "gated_delta_accept: at most 64 nodes, and path entries")
     _need(state.dim() == 4 and state.shape[1:] == (nv, d, d) and state.dtype == torch.float32,
           "gated delta rule: state must be fp32 [n, nv, D, D]")
     _check_out_state(state, out_state)
