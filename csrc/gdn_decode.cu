@@ -153,15 +153,29 @@ struct State {
   }
 };
 
-// 16-byte chunks of rows [0, rows) of D channels into shared memory (zeros at and beyond
-// `live`) and 1 / sqrt(|row|^2 + 1e-6) of each.
+// Rows [0, rows) of D channels into shared memory, asynchronously; zeros at and beyond `live`
+// (`live` >= 1).
 template <int D, int ST>
-__device__ __forceinline__ void load_rows(const bf16* src, int64_t ts, int live, int rows, bf16* dst, float* inv) {
-  constexpr int L = D / 8;  // lanes of one row
-  for (int i = threadIdx.x; i < (rows * L + 31) / 32 * 32; i += blockDim.x) {
+__device__ __forceinline__ void copy_rows(const bf16* src, int64_t ts, int live, int rows, bf16* dst) {
+  constexpr int L = D / 8;  // 16-byte chunks of one row
+  for (int i = threadIdx.x; i < rows * L; i += blockDim.x) {
+    const int r = i / L, c = i % L;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sm100::smem_u32(dst + r * ST + c * 8)),
+                 "l"(src + min(r, live - 1) * ts + c * 8), "r"(r < live ? 16 : 0)
+                 : "memory");
+  }
+}
+
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// 1 / sqrt(|row|^2 + 1e-6) of rows in shared memory, D / 8 lanes a row.
+template <int D, int ST>
+__device__ __forceinline__ void row_norms(const bf16* rows, int n, float* inv) {
+  constexpr int L = D / 8;
+  for (int i = threadIdx.x; i < (n * L + 31) / 32 * 32; i += blockDim.x) {
     const int r = i / L, c = i % L;
     uint4 w = make_uint4(0, 0, 0, 0);
-    if (r < live) w = *reinterpret_cast<const uint4*>(src + r * ts + c * 8);
+    if (r < n) w = *reinterpret_cast<const uint4*>(rows + r * ST + c * 8);
     const uint32_t in[4] = {w.x, w.y, w.z, w.w};
     float ss = 0.f;
 #pragma unroll
@@ -171,11 +185,17 @@ __device__ __forceinline__ void load_rows(const bf16* src, int64_t ts, int live,
     }
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffff, ss, o);
-    if (r < rows) {
-      *reinterpret_cast<uint4*>(dst + r * ST + c * 8) = w;
-      if (c == 0) inv[r] = rsqrtf(ss + 1e-6f);
-    }
+    if (r < n && c == 0) inv[r] = rsqrtf(ss + 1e-6f);
   }
+}
+
+// x = hi + lo in bf16 (16 bits), for a pair of values
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  const float2 hf = __bfloat1622float2(h);
+  const __nv_bfloat162 l = __floats2bfloat162_rn(x - hf.x, y - hf.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
 // ------------------------------------------------------------------ nodes (a tree, or tokens in chunks)
@@ -187,11 +207,9 @@ struct Nodes {
   static constexpr int KST = D + 8;                    // row strides: 4 banks apart
   static constexpr int US = COLS + 4;
   static constexpr int MS = TP + 4;
+  static constexpr int AS = TP + 8;                    // words of a row of node pairs (8 banks apart)
   static constexpr int ROWS = TP * KST * 2;            // bytes of K or Q
-  static constexpr int YB = TP * US * 4;               // bytes of U or Y
-  static constexpr int QY = ROWS > YB ? ROWS : YB;     // Q, then Y
-  static constexpr int SMEM = ROWS + QY + YB + 2 * TP * MS * 4 + 8 * TP * 4;
-  static constexpr int BLK = TP < 16 ? TP : 16;
+  static constexpr int SMEM = 2 * ROWS + TP * US * 4 + TP * MS * 4 + TP * AS * 4 + 8 * TP * 4;
 };
 
 // TREE: T <= 8 NT nodes with parents; the state is only read. Otherwise tokens in chunks of
@@ -199,15 +217,14 @@ struct Nodes {
 template <int D, int NT, bool TREE>
 __global__ void __launch_bounds__(Nodes<D, NT>::THREADS, 3) gdn_nodes_kernel(Args a) {
   using C = Nodes<D, NT>;
-  constexpr int TP = C::TP, TN = 8 * NT, KST = C::KST, US = C::US, MS = C::MS, COLS = C::COLS, SL = D / COLS;
+  constexpr int TP = C::TP, TN = 8 * NT, KST = C::KST, US = C::US, MS = C::MS, AS = C::AS, COLS = C::COLS, SL = D / COLS;
   extern __shared__ __align__(16) uint8_t sm[];
   bf16* ks = reinterpret_cast<bf16*>(sm);               // [TP][KST]
-  bf16* qs = reinterpret_cast<bf16*>(sm + C::ROWS);     // [TP][KST]
-  float* ys = reinterpret_cast<float*>(sm + C::ROWS);   // [TP][US], once Q is consumed
-  float* us = reinterpret_cast<float*>(sm + C::ROWS + C::QY);  // [TP][US] right-hand sides, then u
+  bf16* qs = ks + TP * KST;                             // [TP][KST]
+  float* us = reinterpret_cast<float*>(qs + TP * KST);  // [TP][US] right-hand sides, then u
   float* mt = us + TP * US;                             // [a][t] decays D[t, a], then M
-  float* at = mt + TP * MS;                             // [a][t] A
-  float* ik = at + TP * MS;                             // [TP] 1 / |k|
+  uint32_t* at = reinterpret_cast<uint32_t*>(mt + TP * MS);  // [2][a / 2][t] A: bf16 pairs, high and low parts
+  float* ik = reinterpret_cast<float*>(at + TP * C::AS);  // [TP] 1 / |k|
   float* iq = ik + TP;                                  // [TP] D^-1/2 / |q|
   float* eg = iq + TP;                                  // [TP] e^g
   float* be = eg + TP;                                  // [TP] beta
@@ -232,8 +249,11 @@ __global__ void __launch_bounds__(Nodes<D, NT>::THREADS, 3) gdn_nodes_kernel(Arg
     const bf16* kp = a.k + s * a.k_bs + t0 * a.k_ts + hk * a.k_hs;
     const bf16* qp = a.q + s * a.q_bs + t0 * a.q_ts + hk * a.q_hs;
     const bf16* vp = a.v + s * a.v_bs + t0 * a.v_ts + h * a.v_hs + col0 + 2 * g;
-    // v of this thread's accumulators, early
-    uint32_t v[NT][2];
+    // everything from global memory is asked for before anything is waited for
+    if (t0 > 0) __syncthreads();  // the previous chunk's readers
+    copy_rows<D, KST>(kp, a.k_ts, n, TP, ks);
+    copy_rows<D, KST>(qp, a.q_ts, n, TP, qs);
+    uint32_t v[NT][2];  // v of this thread's accumulators
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -241,13 +261,10 @@ __global__ void __launch_bounds__(Nodes<D, NT>::THREADS, 3) gdn_nodes_kernel(Arg
         const int t = 8 * j + 2 * q + i;
         v[j][i] = t < n ? *reinterpret_cast<const uint32_t*>(vp + t * a.v_ts) : 0u;
       }
-    if (t0 > 0) __syncthreads();  // the previous chunk's readers
-    load_rows<D, KST>(kp, a.k_ts, n, TP, ks, ik);
-    load_rows<D, KST>(qp, a.q_ts, n, TP, qs, iq);
     for (int t = tid; t < TP; t += C::THREADS) {
       const bool in = t < n;
-      eg[t] = in ? expf(a.g[s * a.g_bs + (t0 + t) * a.g_ts + h]) : 1.f;
-      be[t] = in ? bf(a.beta[s * a.b_bs + (t0 + t) * a.b_ts + h]) : 0.f;
+      const float gv = in ? a.g[s * a.g_bs + (t0 + t) * a.g_ts + h] : 0.f;
+      const float bv = in ? bf(a.beta[s * a.b_bs + (t0 + t) * a.b_ts + h]) : 0.f;
       if constexpr (TREE) {
         int p = in ? a.parents[s * a.p_bs + t] : -1;
         if (p < -1 || p >= t) {
@@ -256,11 +273,16 @@ __global__ void __launch_bounds__(Nodes<D, NT>::THREADS, 3) gdn_nodes_kernel(Arg
         }
         par[t] = p;
       }
+      eg[t] = expf(gv);
+      be[t] = bv;
     }
     for (int i = tid; i < TP * MS / 4; i += C::THREADS) reinterpret_cast<float4*>(mt)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if constexpr (TN < TP)  // rows of u that no node fills
       for (int i = tid; i < (TP - TN) * US; i += C::THREADS) us[TN * US + i] = 0.f;
+    copies_done();
     __syncthreads();
+    row_norms<D, KST>(ks, TP, ik);
+    row_norms<D, KST>(qs, TP, iq);
     // decays: a tree's rows walk up to the root, a chain's columns run down
     if constexpr (TREE) {
       for (int t = tid; t < TP; t += C::THREADS) {
@@ -329,40 +351,34 @@ __global__ void __launch_bounds__(Nodes<D, NT>::THREADS, 3) gdn_nodes_kernel(Arg
     if (!TREE) __syncthreads();  // cf before mt changes
     // K K^T and Q K^T on the lower triangle, with their decays: M and A, transposed
     const float rd = rsqrtf((float)D);
-    for (int mi = warp; mi < TP / 16; mi += C::THREADS / 32) {
-      for (int nj = 0; nj <= 2 * mi + 1; ++nj) {
-        float kk4[4] = {}, qk4[4] = {};
+    for (int x = warp; x < TP / 16 * (TP / 16 + 1); x += C::THREADS / 32) {  // tiles of 16 x 8
+      int mi = 0;
+      while ((mi + 1) * (mi + 2) <= x) ++mi;
+      const int nj = x - mi * (mi + 1);
+      float kk4[4] = {}, qk4[4] = {};
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const bf16* ar = ks + (16 * mi + g) * KST + 16 * kk + 2 * q;
-          const bf16* aq = qs + (16 * mi + g) * KST + 16 * kk + 2 * q;
-          const bf16* br = ks + (8 * nj + g) * KST + 16 * kk + 2 * q;
-          auto u32 = [](const bf16* p) { return *reinterpret_cast<const uint32_t*>(p); };
-          const uint32_t b0 = u32(br), b1 = u32(br + 8);
-          const uint32_t fa[4] = {u32(ar), u32(ar + 8 * KST), u32(ar + 8), u32(ar + 8 * KST + 8)};
-          const uint32_t fq[4] = {u32(aq), u32(aq + 8 * KST), u32(aq + 8), u32(aq + 8 * KST + 8)};
-          mma16816(kk4, fa, b0, b1);
-          mma16816(qk4, fq, b0, b1);
-        }
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const bf16* ar = ks + (16 * mi + g) * KST + 16 * kk + 2 * q;
+        const bf16* aq = qs + (16 * mi + g) * KST + 16 * kk + 2 * q;
+        const bf16* br = ks + (8 * nj + g) * KST + 16 * kk + 2 * q;
+        auto u32 = [](const bf16* p) { return *reinterpret_cast<const uint32_t*>(p); };
+        const uint32_t b0 = u32(br), b1 = u32(br + 8);
+        const uint32_t fa[4] = {u32(ar), u32(ar + 8 * KST), u32(ar + 8), u32(ar + 8 * KST + 8)};
+        const uint32_t fq[4] = {u32(aq), u32(aq + 8 * KST), u32(aq + 8), u32(aq + 8 * KST + 8)};
+        mma16816(kk4, fa, b0, b1);
+        mma16816(qk4, fq, b0, b1);
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = 16 * mi + g + (i >> 1) * 8, c = 8 * nj + 2 * q + (i & 1);
-          const float d = mt[c * MS + t] * ik[c];
-          at[c * MS + t] = d * iq[t] * rd * qk4[i];
-          mt[c * MS + t] = c < t ? d * ik[t] * be[t] * kk4[i] : 0.f;
-        }
+      for (int i = 0; i < 4; i += 2) {
+        const int t = 16 * mi + g + (i >> 1) * 8, c = 8 * nj + 2 * q;
+        const float d0 = mt[c * MS + t] * ik[c], d1 = mt[(c + 1) * MS + t] * ik[c + 1];
+        const float sq = iq[t] * rd, sk = ik[t] * be[t];
+        split2(d0 * sq * qk4[i], d1 * sq * qk4[i + 1], at[(c >> 1) * AS + t], at[(TP / 2 + (c >> 1)) * AS + t]);
+        mt[c * MS + t] = c < t ? d0 * sk * kk4[i] : 0.f;
+        mt[(c + 1) * MS + t] = c + 1 < t ? d1 * sk * kk4[i + 1] : 0.f;
       }
     }
     __syncthreads();
-    // Q is consumed: its place takes w S^T q^
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int t = 8 * j + 2 * q + i;
-        const float w = wt[t] * iq[t] * rd;
-        *reinterpret_cast<float2*>(ys + t * US + 16 * warp + 2 * g) = make_float2(w * qa[j][i], w * qa[j][2 + i]);
-      }
     // (I + M) u = right-hand side, by blocks of 16 nodes; thread = (value channel, half of the rows)
     const int c = tid % COLS, half = tid / COLS;
     constexpr int R = TN < 16 ? TN / 2 : 8;  // rows of one thread
@@ -404,29 +420,50 @@ __global__ void __launch_bounds__(Nodes<D, NT>::THREADS, 3) gdn_nodes_kernel(Arg
       }
       __syncthreads();
     }
-    // o = w S^T q^ + A u
-    for (int r = half * R; r < TN; r += 2 * R) {
-      if (r >= n) break;
-      float x[R];
+    // o = w S^T q^ + A u, in the accumulators of S^T Q^T. Two parts (16 bits) of u and of A are
+    // plenty for an output of bf16.
 #pragma unroll
-      for (int i = 0; i < R; ++i) x[i] = ys[(r + i) * US + c];
-#pragma unroll 4
-      for (int m = 0; m < r + R; ++m) {
-        const float u = us[m * US + c];
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int i = 0; i < R; i += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(at + m * MS + r + i);
-          x[i] = fmaf(f.x, u, x[i]), x[i + 1] = fmaf(f.y, u, x[i + 1]);
-          x[i + 2] = fmaf(f.z, u, x[i + 2]), x[i + 3] = fmaf(f.w, u, x[i + 3]);
-        }
+      for (int i = 0; i < 2; ++i) {
+        const float w = wt[8 * j + 2 * q + i] * iq[8 * j + 2 * q + i] * rd;
+        qa[j][i] *= w;
+        qa[j][2 + i] *= w;
       }
 #pragma unroll
-      for (int i = 0; i < R; ++i)
-        if (r + i < n) {
-          a.out[ob + (t0 + r + i) * ots + c] = __float2bfloat16(x[i]);
-          if constexpr (TREE) a.u[ob + (r + i) * ots + c] = us[(r + i) * US + c];
-        }
+    for (int b = 0; b < TP / 16; ++b) {  // 16 nodes a
+      uint32_t f[2][4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float* up = us + (16 * b + 8 * x + 2 * q) * US + 16 * warp + 2 * g;
+        const float2 u0 = *reinterpret_cast<const float2*>(up), u1 = *reinterpret_cast<const float2*>(up + US);
+        split2(u0.x, u1.x, f[0][2 * x], f[1][2 * x]);
+        split2(u0.y, u1.y, f[0][2 * x + 1], f[1][2 * x + 1]);
+      }
+#pragma unroll
+      for (int j = 2 * b; j < NT; ++j) {  // nodes t at or after them
+        const uint32_t* hp = at + (8 * b + q) * AS + 8 * j + g;
+        const uint32_t* lp = hp + TP / 2 * AS;
+        const uint32_t h0 = hp[0], h1 = hp[4 * AS];
+        mma16816(qa[j], f[1], h0, h1);
+        mma16816(qa[j], f[0], lp[0], lp[4 * AS]);
+        mma16816(qa[j], f[0], h0, h1);
+      }
     }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int t = 8 * j + 2 * q + i;
+        if (t < n)
+          *reinterpret_cast<__nv_bfloat162*>(a.out + ob + (t0 + t) * ots + 16 * warp + 2 * g) =
+              __floats2bfloat162_rn(qa[j][i], qa[j][2 + i]);
+      }
+    if constexpr (TREE)
+      for (int i = tid; i < n * COLS / 4; i += C::THREADS) {
+        const int t = i / (COLS / 4), x = i % (COLS / 4) * 4;
+        *reinterpret_cast<float4*>(a.u + ob + t * ots + x) = *reinterpret_cast<const float4*>(us + t * US + x);
+      }
     if constexpr (!TREE) {
       S.scale(wt[TP - 1]);
 #pragma unroll 1
