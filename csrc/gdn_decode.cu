@@ -566,6 +566,171 @@ __global__ void __launch_bounds__(Nodes<D, 2>::THREADS) gdn_accept_kernel(Args a
   S.store(a.out_state + row * a.o_rs + (int64_t)h * D * D + cs + 16 * warp, g, q);
 }
 
+// ------------------------------------------------------------------ one token; short paths
+// Plain loads and FMAs where a state's elements meet few nodes: a warp takes 32 value
+// channels of a head on its own (lanes of a row group hold 4 channels each, a group D / GR key
+// channels), so nothing but its own loads is waited for and 12 warps keep 190 KB an SM under way.
+template <int D>
+struct Slice {
+  static constexpr int CW = D < 32 ? D : 32;   // value channels of a warp
+  static constexpr int LR = CW / 4;            // lanes of one row
+  static constexpr int GR = 32 / LR;           // row groups
+  static constexpr int N = D / GR;             // key channels of a lane: [group N, group N + N)
+  static constexpr int WARPS = 2;              // of a CTA
+};
+
+// D bf16 channels into fp32 shared memory by one warp; returns 1 / sqrt(|x|^2 + 1e-6).
+template <int D>
+__device__ __forceinline__ float warp_row(const bf16* x, float* dst, int lane) {
+  float ss = 0.f;
+#pragma unroll
+  for (int i = lane * 2; i < D; i += 64) {
+    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(x + i));
+    *reinterpret_cast<float2*>(dst + i) = f;
+    ss = fmaf(f.x, f.x, fmaf(f.y, f.y, ss));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffff, ss, o);
+  return rsqrtf(ss + 1e-6f);
+}
+
+template <int D>
+__global__ void __launch_bounds__(Slice<D>::WARPS * 32) gdn_step_kernel(Args a, int slices) {
+  using C = Slice<D>;
+  constexpr int N = C::N;
+  __shared__ __align__(16) float kq[C::WARPS][2][D];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int x = blockIdx.x * C::WARPS + warp;  // (head, slice)
+  if (x >= slices) return;
+  const int h = x / (D / C::CW), s = blockIdx.y, hk = h / a.groups;
+  const int col = x % (D / C::CW) * C::CW + lane % C::LR * 4, k0 = lane / C::LR * N;
+  const int64_t row = a.rows ? a.rows[s] : s;
+  const bool valid = row >= 0 && row < a.n;
+  if (!valid && row != -1 && lane == 0) atomicExch(a.err, ERR_INDEX);
+  const int64_t at = (int64_t)h * D * D + (int64_t)k0 * D + col;
+  float4 S[N];
+  if (valid) {
+    const float* st = a.state + row * a.s_rs + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i) S[i] = *reinterpret_cast<const float4*>(st + i * D);
+  }
+  const int cnt = a.counts ? a.counts[s] : 1;
+  if ((cnt < 0 || cnt > 1) && lane == 0) atomicExch(a.err, ERR_INDEX);
+  const bool live = valid && cnt > 0;
+  float o[4] = {};
+  if (live) {
+    const uint2 vr = *reinterpret_cast<const uint2*>(a.v + s * a.v_bs + h * a.v_hs + col);
+    const float eg = expf(a.g[s * a.g_bs + h]), be = bf(a.beta[s * a.b_bs + h]);
+    const float ik = warp_row<D>(a.k + s * a.k_bs + hk * a.k_hs, kq[warp][0], lane);
+    const float iq = warp_row<D>(a.q + s * a.q_bs + hk * a.q_hs, kq[warp][1], lane) * rsqrtf((float)D);
+    __syncwarp();
+    const float* ks = kq[warp][0] + k0;
+    const float* qs = kq[warp][1] + k0;
+    float xk[4] = {}, xq[4] = {}, dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float k = ks[i], q = qs[i];
+      xk[0] = fmaf(k, S[i].x, xk[0]), xk[1] = fmaf(k, S[i].y, xk[1]);
+      xk[2] = fmaf(k, S[i].z, xk[2]), xk[3] = fmaf(k, S[i].w, xk[3]);
+      xq[0] = fmaf(q, S[i].x, xq[0]), xq[1] = fmaf(q, S[i].y, xq[1]);
+      xq[2] = fmaf(q, S[i].z, xq[2]), xq[3] = fmaf(q, S[i].w, xq[3]);
+      dot = fmaf(k, q, dot);
+    }
+#pragma unroll
+    for (int w = C::LR; w < 32; w <<= 1) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        xk[c] += __shfl_xor_sync(0xffffffff, xk[c], w);
+        xq[c] += __shfl_xor_sync(0xffffffff, xq[c], w);
+      }
+      dot += __shfl_xor_sync(0xffffffff, dot, w);
+    }
+    const float v[4] = {__uint_as_float(vr.x << 16), __uint_as_float(vr.x & 0xffff0000u), __uint_as_float(vr.y << 16),
+                        __uint_as_float(vr.y & 0xffff0000u)};
+    float u[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      u[c] = be * (v[c] - eg * ik * xk[c]);
+      o[c] = iq * fmaf(eg, xq[c], dot * ik * u[c]);
+      u[c] *= ik;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float k = ks[i];
+      S[i].x = fmaf(k, u[0], eg * S[i].x), S[i].y = fmaf(k, u[1], eg * S[i].y);
+      S[i].z = fmaf(k, u[2], eg * S[i].z), S[i].w = fmaf(k, u[3], eg * S[i].w);
+    }
+  }
+  if (lane < C::LR) {
+    __nv_bfloat162 w[2] = {__floats2bfloat162_rn(o[0], o[1]), __floats2bfloat162_rn(o[2], o[3])};
+    *reinterpret_cast<uint2*>(a.out + ((int64_t)s * a.nv + h) * D + col) = *reinterpret_cast<const uint2*>(w);
+  }
+  if (valid) {
+    float* so = a.out_state + row * a.o_rs + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<float4*>(so + i * D) = S[i];
+  }
+}
+
+constexpr int SHORT_PATH = 16;
+
+template <int D>
+__global__ void __launch_bounds__(Slice<D>::WARPS * 32) gdn_accept_short_kernel(Args a, int slices) {
+  using C = Slice<D>;
+  constexpr int N = C::N;
+  __shared__ __align__(16) float kr[C::WARPS][2][D];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int x = blockIdx.x * C::WARPS + warp;
+  if (x >= slices) return;
+  const int h = x / (D / C::CW), s = blockIdx.y, hk = h / a.groups;
+  const int col = x % (D / C::CW) * C::CW + lane % C::LR * 4, k0 = lane / C::LR * N;
+  const int64_t row = a.rows ? a.rows[s] : s;
+  if (row < 0 || row >= a.n) {
+    if (row != -1 && lane == 0) atomicExch(a.err, ERR_INDEX);
+    return;
+  }
+  const int64_t at = (int64_t)h * D * D + (int64_t)k0 * D + col;
+  const float* st = a.state + row * a.s_rs + at;
+  float4 S[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) S[i] = *reinterpret_cast<const float4*>(st + i * D);
+  // lane j: node j of the path, its decay, and the product of the later ones
+  int node = lane < a.m ? a.path[(int64_t)s * a.m + lane] : -1;
+  if (node < -1 || node >= a.T) {
+    atomicExch(a.err, ERR_INDEX);
+    node = -1;
+  }
+  float after = node >= 0 ? expf(a.g[s * a.g_bs + node * a.g_ts + h]) : 1.f;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float y = __shfl_down_sync(0xffffffff, after, o);
+    if (lane + o < 32) after *= y;
+  }
+  const float gamma = __shfl_sync(0xffffffff, after, 0);
+  after = __shfl_down_sync(0xffffffff, after, 1);  // (lane 31 is beyond a short path)
+#pragma unroll
+  for (int i = 0; i < N; ++i) S[i].x *= gamma, S[i].y *= gamma, S[i].z *= gamma, S[i].w *= gamma;
+  uint32_t left = __ballot_sync(0xffffffff, node >= 0);
+  for (int b = 0; left; b ^= 1, left &= left - 1) {
+    const int j = __ffs(left) - 1, t = __shfl_sync(0xffffffff, node, j);
+    const float f = __shfl_sync(0xffffffff, after, j);
+    const float4 ur = *reinterpret_cast<const float4*>(a.u_in + (((int64_t)s * a.T + t) * a.nv + h) * D + col);
+    const float w = warp_row<D>(a.k + s * a.k_bs + t * a.k_ts + hk * a.k_hs, kr[warp][b], lane) * f;
+    __syncwarp();
+    const float* ks = kr[warp][b] + k0;
+    const float4 u = make_float4(ur.x * w, ur.y * w, ur.z * w, ur.w * w);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float k = ks[i];
+      S[i].x = fmaf(k, u.x, S[i].x), S[i].y = fmaf(k, u.y, S[i].y);
+      S[i].z = fmaf(k, u.z, S[i].z), S[i].w = fmaf(k, u.w, S[i].w);
+    }
+  }
+  float* so = a.out_state + row * a.o_rs + at;
+#pragma unroll
+  for (int i = 0; i < N; ++i) *reinterpret_cast<float4*>(so + i * D) = S[i];
+}
+
 template <int D, int NT, bool TREE>
 void launch_nodes(const Args& a, int64_t b) {
   using C = Nodes<D, NT>;
@@ -577,9 +742,16 @@ void launch_nodes(const Args& a, int64_t b) {
 }
 
 // the fewest nodes per pass that hold T (chunks of 64 beyond)
+template <int D>
+dim3 slice_grid(int nv, int64_t b) {
+  return dim3((unsigned)((nv * (D / Slice<D>::CW) + Slice<D>::WARPS - 1) / Slice<D>::WARPS), (unsigned)b);
+}
+
 template <int D, bool TREE>
 void launch_for(const Args& a, int64_t b) {
-  if (a.T <= 8)
+  if (!TREE && a.T == 1)
+    gdn_step_kernel<D><<<slice_grid<D>(a.nv, b), Slice<D>::WARPS * 32, 0, stream()>>>(a, a.nv * (D / Slice<D>::CW));
+  else if (a.T <= 8)
     launch_nodes<D, 1, TREE>(a, b);
   else if (a.T <= 16)
     launch_nodes<D, 2, TREE>(a, b);
@@ -587,6 +759,15 @@ void launch_for(const Args& a, int64_t b) {
     launch_nodes<D, 4, TREE>(a, b);
   else
     launch_nodes<D, 8, TREE>(a, b);
+}
+
+template <int D>
+void launch_accept(const Args& a, int64_t b) {
+  if (a.m <= SHORT_PATH)
+    gdn_accept_short_kernel<D><<<slice_grid<D>(a.nv, b), Slice<D>::WARPS * 32, 0, stream()>>>(a, a.nv * (D / Slice<D>::CW));
+  else
+    gdn_accept_kernel<D><<<dim3((unsigned)(a.nv * (D / Nodes<D, 2>::COLS)), (unsigned)b), Nodes<D, 2>::THREADS, 0,
+                           stream()>>>(a);
 }
 
 }  // namespace gdnd
@@ -732,10 +913,7 @@ void gdn_accept(at::Tensor k, at::Tensor g, at::Tensor u, at::Tensor path, at::T
   d.a.path = path.data_ptr<int>();
   d.a.T = (int)d.T, d.a.m = (int)path.size(1), d.a.nv = (int)d.nv, d.a.groups = (int)groups;
   d.a.err = device_error_flag();
-#define NS_X(DD)                                                                                       \
-  gdnd::gdn_accept_kernel<DD>                                                                          \
-      <<<dim3((unsigned)(d.nv * (DD / gdnd::Nodes<DD, 2>::COLS)), (unsigned)d.b), gdnd::Nodes<DD, 2>::THREADS, 0, \
-         stream()>>>(d.a);
+#define NS_X(DD) gdnd::launch_accept<DD>(d.a, d.b);
   NS_GDN_CASES(d.D, NS_X)
 #undef NS_X
   NS_CUDA(cudaGetLastError());

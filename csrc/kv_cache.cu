@@ -39,56 +39,73 @@ struct WriteArgs {
   void* pool[2];
   uint8_t* exps[2];
   const int64_t* slots;
-  int64_t n, pages;
-  int heads, page, d;
+  int64_t slots_end;
+  int n, heads, page_log2, d;
   int* err;
 };
 
-// One warp per (token, head) row of K (blockIdx.y = 0) or V (1); lane l holds channels
-// [8l, 8l + 8).
-template <bool E4M3>
+// 16 channels per thread, G (a power of two) neighbouring lanes per (token, head) row of K
+// (blockIdx.y = 0) or V (1); two rows per thread, so that two rows' loads are under way.
+template <bool E4M3, int G>
 __global__ void __launch_bounds__(256) cache_write_kernel(WriteArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, which = blockIdx.y;
-  if (row >= a.n * a.heads) return;
-  const int64_t tok = row / a.heads;
-  const int h = (int)(row % a.heads);
-  const int64_t slot = a.slots[tok];
-  if (slot < 0 || slot >= a.pages * a.page) {
-    if (slot != -1 && lane == 0) atomicExch(a.err, ERR_INDEX);
-    return;
+  const int which = blockIdx.y, c = threadIdx.x % G * 16;
+  const unsigned r0 = blockIdx.x * (512 / G) + threadIdx.x / G, rows = (unsigned)a.n * a.heads;
+  uint4 w[2][2];
+  int64_t dst[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const unsigned r = r0 + i * (256 / G);
+    dst[i] = -1;
+    w[i][0] = w[i][1] = make_uint4(0, 0, 0, 0);
+    if (r < rows) {
+      const unsigned tok = r / a.heads, h = r % a.heads;
+      const int64_t slot = a.slots[tok];
+      if (slot >= 0 && slot < a.slots_end)
+        dst[i] = ((((slot >> a.page_log2) * a.heads + h) << a.page_log2) + (slot & ((1 << a.page_log2) - 1)));
+      else if (slot != -1 && c == 0)
+        atomicExch(a.err, ERR_INDEX);
+      if (dst[i] >= 0 && c < a.d) {
+        const uint4* x = reinterpret_cast<const uint4*>(a.x[which] + tok * a.x_ts[which] + h * a.x_hs[which] + c);
+        w[i][0] = x[0];
+        w[i][1] = x[1];
+      }
+    }
   }
-  const int64_t dst = ((slot / a.page) * a.heads + h) * a.page + slot % a.page;
-  const bool on = lane * 8 < a.d;
-  uint4 raw = make_uint4(0, 0, 0, 0);
-  if (on) raw = *reinterpret_cast<const uint4*>(a.x[which] + tok * a.x_ts[which] + h * a.x_hs[which] + lane * 8);
-  if constexpr (!E4M3) {
-    if (on) *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.pool[which]) + dst * a.d + lane * 8) = raw;
-  } else {
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    float x[8];
-    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t b = (i & 1) ? (w[i / 2] & 0xffff0000u) : (w[i / 2] << 16);
-      x[i] = __uint_as_float(b);
-      const uint32_t m = b & 0x7fffffffu;
-      top = max(top, m < 0x7f800000u ? m : 0u);  // infinities and NaN do not count
-    }
-    top = __reduce_max_sync(0xffffffff, top);
-    const int e = row_exponent(top);
-    const float s = pow2(-e);
-    uint32_t code[2] = {0, 0};
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (!E4M3) {
+      if (dst[i] >= 0 && c < a.d) {
+        uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.pool[which]) + dst[i] * a.d + c);
+        o[0] = w[i][0];
+        o[1] = w[i][1];
+      }
+    } else {
+      const uint32_t in[8] = {w[i][0].x, w[i][0].y, w[i][0].z, w[i][0].w, w[i][1].x, w[i][1].y, w[i][1].z, w[i][1].w};
+      uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const __nv_fp8x2_storage_t c =
-          __nv_cvt_float2_to_fp8x2(make_float2(x[i] * s, x[i + 1] * s), __NV_SATFINITE, __NV_E4M3);
-      code[i / 4] |= (uint32_t)c << (8 * (i & 3));
+      for (int j = 0; j < 8; ++j) {  // infinities and NaN do not count
+        const uint32_t lo = (in[j] << 16) & 0x7fffffffu, hi = in[j] & 0x7fff0000u;
+        top = max(top, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
+      }
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffff, top, o));
+      const int e = row_exponent(top);
+      const float s = pow2(-e);
+      uint32_t code[4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const __nv_fp8x2_storage_t p = __nv_cvt_float2_to_fp8x2(
+            make_float2(__uint_as_float(in[j] << 16) * s, __uint_as_float(in[j] & 0xffff0000u) * s), __NV_SATFINITE,
+            __NV_E4M3);
+        code[j / 2] = j & 1 ? code[j / 2] | (uint32_t)p << 16 : (uint32_t)p;
+      }
+      if (dst[i] >= 0) {
+        if (c < a.d)
+          *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.pool[which]) + dst[i] * a.d + c) =
+              make_uint4(code[0], code[1], code[2], code[3]);
+        if (c == 0) a.exps[which][dst[i]] = (uint8_t)(e + EXP_BIAS);
+      }
     }
-    if (on)
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.pool[which]) + dst * a.d + lane * 8) =
-          make_uint2(code[0], code[1]);
-    if (lane == 0) a.exps[which][dst] = (uint8_t)(e + EXP_BIAS);
   }
 }
 
@@ -97,54 +114,71 @@ struct ReadArgs {
   const uint8_t* exps[2];
   bf16* out[2];
   const int *table, *lens, *starts;
-  int64_t b, length, pages, max_pages;
-  int heads, page, d;
+  int length, pages, max_pages, heads, page_log2, d, per;
   int* err;
 };
 
-// One thread per 8 channels of (sequence, position, head) of K (blockIdx.y = 0) or V (1).
+constexpr int READ_POS = 32;  // positions of one CTA
+
+// CTA: 32 positions of one sequence, K or V (blockIdx.z). Thread: 16 channels of one head at
+// every `per`-th position; neighbouring threads write neighbouring bytes.
 template <bool E4M3>
 __global__ void __launch_bounds__(256) cache_read_kernel(ReadArgs a) {
-  const int cols = a.d / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int which = blockIdx.y;
-  if (i >= a.b * a.length * a.heads * cols) return;
-  const int c = (int)(i % cols);
-  const int64_t r = i / cols;
-  const int h = (int)(r % a.heads);
-  const int64_t bt = r / a.heads;
-  const int64_t s = bt / a.length;
-  const int64_t pos = bt % a.length + (a.starts ? a.starts[s] : 0);
-  uint4 out = make_uint4(0, 0, 0, 0);
-  const int64_t len = min((int64_t)a.lens[s], a.max_pages * a.page);
-  if (c == 0 && h == 0 && (a.lens[s] != len || len < 0 || pos < 0)) atomicExch(a.err, ERR_INDEX);
-  if (pos >= 0 && pos < len) {
-    const int64_t pg = a.table[s * a.max_pages + pos / a.page];
-    if (pg < 0 || pg >= a.pages) {
-      if (c == 0) atomicExch(a.err, ERR_INDEX);
-    } else {
-      const int64_t src = (pg * a.heads + h) * a.page + pos % a.page;
-      if constexpr (!E4M3) {
-        out = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.pool[which]) + src * a.d + c * 8);
-      } else {
-        const uint2 code =
-            *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(a.pool[which]) + src * a.d + c * 8);
-        const float sc = pow2(min(max((int)a.exps[which][src] - EXP_BIAS, EXP_MIN), EXP_MAX));
-        uint32_t w[4];
+  const int s = blockIdx.y, which = blockIdx.z, cols = a.d / 16, hc = a.heads * cols;
+  const int p0 = blockIdx.x * READ_POS;
+  const int64_t first = a.starts ? a.starts[s] : 0;
+  int64_t len = a.lens[s];
+  const int64_t most = (int64_t)a.max_pages << a.page_log2;
+  if (len < 0 || len > most || first < 0) {
+    if (threadIdx.x == 0) atomicExch(a.err, ERR_INDEX);
+    len = first < 0 ? 0 : min(max(len, (int64_t)0), most);
+  }
+  const int* table = a.table + (int64_t)s * a.max_pages;
+  for (int x0 = threadIdx.x; x0 < hc * a.per; x0 += 256) {
+    const int x = x0 % hc, h = x / cols, c = x % cols * 16;
+    bf16* out = a.out[which] + ((int64_t)s * a.length * a.heads + h) * a.d + c;
+#pragma unroll 4
+    for (int i = x0 / hc; i < READ_POS; i += a.per) {
+      if (p0 + i >= a.length) break;
+      const int64_t pos = first + p0 + i;
+      uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+      if (pos < len) {
+        const int pg = table[pos >> a.page_log2];
+        if (pg < 0 || pg >= a.pages) {
+          atomicExch(a.err, ERR_INDEX);
+        } else {
+          const int64_t src = (((int64_t)pg * a.heads + h) << a.page_log2) + (pos & ((1 << a.page_log2) - 1));
+          if constexpr (!E4M3) {
+            const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.pool[which]) + src * a.d + c);
+            w[0] = p[0];
+            w[1] = p[1];
+          } else {
+            const uint4 code =
+                *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.pool[which]) + src * a.d + c);
+            const float sc = pow2(min(max((int)a.exps[which][src] - EXP_BIAS, EXP_MIN), EXP_MAX));
+            const uint32_t in[4] = {code.x, code.y, code.z, code.w};
+            uint32_t o[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t pair = ((j < 2 ? code.x : code.y) >> (16 * (j & 1))) & 0xffff;
-          const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)pair, __NV_E4M3);
-          const float2 f = __half22float2(__half2(hr));
-          const __nv_bfloat162 o = __floats2bfloat162_rn(f.x * sc, f.y * sc);
-          w[j] = *reinterpret_cast<const uint32_t*>(&o);
+            for (int j = 0; j < 8; ++j) {
+              const uint32_t pair = (in[j / 2] >> (16 * (j & 1))) & 0xffff;
+              const float2 f =
+                  __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)pair, __NV_E4M3)));
+              const __nv_bfloat162 v = __floats2bfloat162_rn(f.x * sc, f.y * sc);
+              o[j] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+            w[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            w[1] = make_uint4(o[4], o[5], o[6], o[7]);
+          }
         }
-        out = make_uint4(w[0], w[1], w[2], w[3]);
       }
+      uint4* o = reinterpret_cast<uint4*>(out + (int64_t)(p0 + i) * a.heads * a.d);
+      o[0] = w[0];
+      o[1] = w[1];
     }
   }
-  *reinterpret_cast<uint4*>(a.out[which] + i * 8) = out;
 }
+
+inline int log2_of(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
 
 }  // namespace kvc
 
@@ -174,19 +208,24 @@ void cache_write(at::Tensor k_pool, at::Tensor v_pool, OptTensor k_exp, OptTenso
   a.pool[1] = v_pool.data_ptr();
   a.exps[0] = const_cast<uint8_t*>(c.ke);
   a.exps[1] = const_cast<uint8_t*>(c.ve);
+  NS_VALUE(rows < (int64_t(1) << 31), "cache_write: too many rows");
   a.slots = slots.data_ptr<int64_t>();
-  a.n = k.size(0);
-  a.pages = c.pages;
+  a.slots_end = c.pages * c.page;
+  a.n = (int)k.size(0);
   a.heads = c.heads;
-  a.page = c.page;
+  a.page_log2 = kvc::log2_of(c.page);
   a.d = c.d;
   a.err = device_error_flag();
-  NS_VALUE((rows + 7) / 8 < (int64_t(1) << 31), "cache_write: too many rows");
-  const dim3 grid((unsigned)((rows + 7) / 8), 2);
-  if (c.e4m3)
-    kvc::cache_write_kernel<true><<<grid, 256, 0, stream()>>>(a);
-  else
-    kvc::cache_write_kernel<false><<<grid, 256, 0, stream()>>>(a);
+#define NS_X(G)                                                                      \
+  {                                                                                  \
+    const dim3 grid((unsigned)((rows + 512 / G - 1) / (512 / G)), 2);                \
+    if (c.e4m3)                                                                      \
+      kvc::cache_write_kernel<true, G><<<grid, 256, 0, stream()>>>(a);               \
+    else                                                                             \
+      kvc::cache_write_kernel<false, G><<<grid, 256, 0, stream()>>>(a);              \
+  }
+  if (c.d <= 64) NS_X(4) else if (c.d <= 128) NS_X(8) else NS_X(16)
+#undef NS_X
   NS_CUDA(cudaGetLastError());
 }
 
@@ -206,24 +245,24 @@ std::vector<at::Tensor> cache_read(at::Tensor k_pool, at::Tensor v_pool, OptTens
   a.table = table.data_ptr<int>();
   auto opt = k_pool.options().dtype(at::kBFloat16);
   at::Tensor ko = at::empty({b, length, c.heads, c.d}, opt), vo = at::empty({b, length, c.heads, c.d}, opt);
-  const int64_t n = b * length * c.heads * (c.d / 8);
-  if (n == 0) return {ko, vo};
+  if (b * length * c.heads == 0) return {ko, vo};
+  NS_VALUE(b < 65536 && length < (int64_t(1) << 31) && table.size(1) < (int64_t(1) << 31),
+           "cache_read: too many sequences or positions");
   a.pool[0] = c.k;
   a.pool[1] = c.v;
   a.exps[0] = c.ke;
   a.exps[1] = c.ve;
   a.out[0] = reinterpret_cast<bf16*>(ko.data_ptr());
   a.out[1] = reinterpret_cast<bf16*>(vo.data_ptr());
-  a.b = b;
-  a.length = length;
-  a.pages = c.pages;
-  a.max_pages = table.size(1);
+  a.length = (int)length;
+  a.pages = (int)c.pages;
+  a.max_pages = (int)table.size(1);
   a.heads = c.heads;
-  a.page = c.page;
+  a.page_log2 = kvc::log2_of(c.page);
   a.d = c.d;
+  a.per = std::max(1, std::min(kvc::READ_POS, 256 / (c.heads * (c.d / 16))));
   a.err = device_error_flag();
-  NS_VALUE((n + 255) / 256 < (int64_t(1) << 31), "cache_read: too many rows");
-  const dim3 grid((unsigned)((n + 255) / 256), 2);
+  const dim3 grid((unsigned)((length + kvc::READ_POS - 1) / kvc::READ_POS), (unsigned)b, 2);
   if (c.e4m3)
     kvc::cache_read_kernel<true><<<grid, 256, 0, stream()>>>(a);
   else
