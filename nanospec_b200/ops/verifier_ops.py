@@ -143,6 +143,23 @@ def causal_attention_gated(q, k, v, gate, cos, sin, rotary_dim):
     return o * gate.sigmoid()
 
 
+def head_norm_partial_rope(x, w, eps, cos, sin, rotary_dim):
+    """(1+w)-RMSNorm of every head, then RoPE on its first ``rotary_dim`` channels.
+
+    x [b, s, H, D] (heads of D contiguous channels, one token stride); cos/sin
+    [b, s, rotary_dim], so every token has a position of its own.
+    """
+    if x.is_cuda:
+        b, s, h, d = x.shape
+        if x.stride(3) != 1 or (b > 1 and x.stride(0) != s * x.stride(1)):
+            x = x.contiguous()
+        out = torch.empty(b, s, h, d, device=x.device, dtype=x.dtype)
+        _c().head_norm_rope(x, h, x.stride(1), x.stride(2), b * s, w, float(eps), cos.reshape(b * s, -1).contiguous(),
+                            sin.reshape(b * s, -1).contiguous(), int(rotary_dim), out)
+        return out
+    return ref.partial_rope(ref.qwen_norm(x, w, eps), cos, sin, rotary_dim)
+
+
 def gated_attention(qg, k, v, q_norm_w, k_norm_w, eps, cos, sin, rotary_dim):
     """The verifier's full-attention mixer after its projections.
 
