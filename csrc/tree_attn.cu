@@ -55,6 +55,7 @@ constexpr float RESCALE_LOG2 = 8.f;   // the reference maximum may lag by this m
 constexpr int V_RESCALE = 4;          // and the reference V exponent by this much
 constexpr float F16_OFFSET = 3.f;     // f16 probabilities are at most 2^(3 + 8 + 4)
 constexpr int SLOT = 16384;           // bytes of one ring slot
+constexpr int SEG_UNITS = 2;          // what beginning and ending a segment costs, in tiles
 constexpr int SOFT_WARPS = 8, CONV_WARPS = 6;
 
 struct Args {
@@ -70,7 +71,7 @@ struct Args {
   float* lse;   // [b, Hq, T]
   float* part;  // [N][2][GT * TPM][D] unnormalised O
   float2* ml;   // [N][2][GT * TPM] reference maximum (log2) and sum
-  int4* info;   // [segments] first CTA, last CTA, workspace slot of the first
+  int2* info;   // [segments] first CTA, last CTA
   int* err;
 };
 
@@ -112,10 +113,14 @@ __device__ __forceinline__ Seq sequence(const Args& a, int s, bool flag) {
   return {len, cnt};
 }
 
-// tiles of a row tile whose first token is live: the prefix and the nodes; one (of zeros) otherwise
+// Units of work: a row tile whose first token is live has the prefix's tiles and the nodes',
+// others one tile of zeros; every segment starts with SEG_UNITS that stand for its beginning
+// and end (q, first loads, output).
+__device__ __forceinline__ int64_t group_units(const Args& a, Seq q, int live) {
+  return (int64_t)live * ((q.len + BN - 1) / BN + 1 + SEG_UNITS) + (int64_t)(a.M - live) * (1 + SEG_UNITS);
+}
 __device__ __forceinline__ int64_t seq_units(const Args& a, Seq q) {
-  const int live = (q.cnt + a.TPM - 1) / a.TPM;
-  return (int64_t)a.Hk * a.HB * (live * ((q.len + BN - 1) / BN + 1) + (a.M - live));
+  return (int64_t)a.Hk * a.HB * group_units(a, q, (q.cnt + a.TPM - 1) / a.TPM);
 }
 
 // A contiguous run of tiles of one segment.
@@ -127,54 +132,68 @@ struct Piece {
   bool whole;
   __device__ __forceinline__ int keys(int t) const { return t < nt ? min(BN, q.len - t * BN) : own; }
   int own;                // keys of the nodes' tile
+  int64_t last;           // the segment's last unit
 };
 
 struct Walk {
-  int s, seg, tile;       // next sequence, segment within it, tile within that
+  int s, seg, off;        // next sequence, segment within it, unit within that
   int64_t unit, end;      // its global number; end of this CTA's run
   Seq q;
+  // the next tiles of one segment; false at the end of the run
   __device__ __forceinline__ bool next(const Args& a, Piece& p) {
-    if (unit >= end) return false;
     const int segs = a.Hk * a.HB * a.M;
-    if (seg == segs) {
-      seg = 0;
-      q = sequence(a, ++s, false);
+    while (unit < end) {
+      if (seg == segs) {
+        seg = 0;
+        q = sequence(a, ++s, false);
+      }
+      p.s = s;
+      p.q = q;
+      p.m = seg % a.M;
+      p.hb = (seg / a.M) % a.HB;
+      p.hk = seg / (a.M * a.HB);
+      p.own = p.m * a.TPM < q.cnt ? q.cnt : 0;
+      p.nt = p.own > 0 ? (q.len + BN - 1) / BN : 0;
+      const int units = p.nt + 1 + SEG_UNITS;
+      p.last = unit - off + units - 1;
+      const int to = (int)min((int64_t)units, off + (end - unit));
+      p.t0 = max(off - SEG_UNITS, 0);
+      p.t1 = max(to - SEG_UNITS, 0);
+      p.whole = p.t0 == 0 && p.t1 == p.nt + 1;
+      unit += to - off;
+      off = to;
+      if (off == units) off = 0, ++seg;
+      if (p.t1 > p.t0) return true;
     }
-    p.s = s;
-    p.q = q;
-    p.m = seg % a.M;
-    p.hb = (seg / a.M) % a.HB;
-    p.hk = seg / (a.M * a.HB);
-    p.nt = p.m * a.TPM < q.cnt ? (q.len + BN - 1) / BN : 0;
-    p.own = p.m * a.TPM < q.cnt ? q.cnt : 0;
-    p.t0 = tile;
-    p.t1 = (int)min((int64_t)p.nt + 1, tile + (end - unit));
-    p.whole = p.t0 == 0 && p.t1 == p.nt + 1;
-    unit += p.t1 - p.t0;
-    tile = p.t1;
-    if (tile == p.nt + 1) tile = 0, ++seg;
-    return true;
+    return false;
   }
 };
 
 // First position and end of CTA blockIdx.x (warp-wide); total tiles in U, working CTAs in N
 // (each has a tile at least).
 __device__ __forceinline__ Walk plan(const Args& a, int lane, int64_t& U, int& N) {
-  int64_t sum = 0;
-  for (int s = lane; s < a.b; s += 32) sum += seq_units(a, sequence(a, s, blockIdx.x == 0));
+  int64_t sum = 0, n = 0;
+  Seq q{0, 0};
+  for (int s = lane; s < a.b; s += 32) {
+    q = sequence(a, s, blockIdx.x == 0);
+    n = seq_units(a, q);
+    sum += n;
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffff, sum, o);
   U = sum;
-  Walk w;
   N = (int)min((int64_t)gridDim.x, U);
+  Walk w;
   w.unit = U * min((int)blockIdx.x, N) / N;
   w.end = U * min((int)blockIdx.x + 1, N) / N;
   int64_t before = 0;
-  w.s = a.b, w.seg = w.tile = 0, w.q = {0, 0};
+  w.s = a.b, w.seg = w.off = 0, w.q = {0, 0};
   for (int s0 = 0; s0 < a.b; s0 += 32) {
     const int s = s0 + lane;
-    const Seq q = s < a.b ? sequence(a, s, false) : Seq{0, 0};
-    const int64_t n = s < a.b ? seq_units(a, q) : 0;
+    if (a.b > 32) {  // (otherwise each lane still has its sequence)
+      q = s < a.b ? sequence(a, s, false) : Seq{0, 0};
+      n = s < a.b ? seq_units(a, q) : 0;
+    }
     int64_t inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -189,15 +208,17 @@ __device__ __forceinline__ Walk plan(const Args& a, int lane, int64_t& U, int& N
       w.q.len = __shfl_sync(0xffffffff, q.len, l);
       w.q.cnt = __shfl_sync(0xffffffff, q.cnt, l);
       const int live = (w.q.cnt + a.TPM - 1) / a.TPM;
-      const int64_t tiles = (w.q.len + BN - 1) / BN + 1;
-      const int64_t group = live * tiles + (a.M - live);  // one (key head, head block)
+      const int64_t units = (w.q.len + BN - 1) / BN + 1 + SEG_UNITS;
+      const int64_t group = group_units(a, w.q, live);  // one (key head, head block)
       w.seg = (int)(rem / group) * a.M;
       rem %= group;
-      if (rem < live * tiles) {
-        w.seg += (int)(rem / tiles);
-        w.tile = (int)(rem % tiles);
+      if (rem < live * units) {
+        w.seg += (int)(rem / units);
+        w.off = (int)(rem % units);
       } else {
-        w.seg += live + (int)(rem - live * tiles);
+        rem -= live * units;
+        w.seg += live + (int)(rem / (1 + SEG_UNITS));
+        w.off = (int)(rem % (1 + SEG_UNITS));
       }
       break;
     }
@@ -351,6 +372,8 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 1);
   static_assert(2 * (NK + NR + NV + FAC) + 9 + 1 <= 64, "barrier area");
 
+  // the join may be set up now; it waits for this kernel's end
+  asm volatile("griddepcontrol.launch_dependents;");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int64_t U;
   int N;
@@ -661,21 +684,30 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
       float rs = a.scale_log2;  // multiplies the products of this row
       if constexpr (E4M3) {
         // q row -> e4m3 and e5m2 rows with a power-of-two scale (the previous piece's products are
-        // complete: this thread has seen all of its scores)
-        if (live) {
-          const bf16* q = a.q + p.s * a.q_bs + tok * a.q_ts + hq * a.q_hs;
+        // complete: this thread has seen all of its scores); this thread's half in one round of loads
+        if (warp_on) {
+          uint4 w[DT / 16];
+          const bf16* q = a.q + p.s * a.q_bs + tok * a.q_ts + hq * a.q_hs + half * (DT / 2);
           uint32_t top = 0;
-#pragma unroll 4
-          for (int c = 0; c < a.D / 8; ++c) top = max(top, finite_top(*reinterpret_cast<const uint4*>(q + c * 8)));
+#pragma unroll
+          for (int c = 0; c < DT / 16; ++c) {
+            w[c] = make_uint4(0, 0, 0, 0);
+            if (live && half * (DT / 2) + c * 8 < a.D) w[c] = *reinterpret_cast<const uint4*>(q + c * 8);
+          }
+#pragma unroll
+          for (int c = 0; c < DT / 16; ++c) top = max(top, finite_top(w[c]));
+          top = max(top, __float_as_uint(exchange(xsum + (pc & 1 ^ 1) * 2 * BM, __uint_as_float(top))));
           const int e = row_exponent(top, 7);
           rs *= pow2(e);
-#pragma unroll 2
-          for (int c = half * (DT / 16); c < (half + 1) * (DT / 16); ++c) {
-            uint2 hi = make_uint2(0, 0), lo = make_uint2(0, 0);
-            if (c * 8 < a.D) split_fp8(*reinterpret_cast<const uint4*>(q + c * 8), pow2(-e), hi, lo);
-            const uint32_t at = tile_offset(BM, row, c >> 1) + (c & 1) * 8;
-            *reinterpret_cast<uint2*>(sQ + at) = hi;
-            *reinterpret_cast<uint2*>(sQ + BM * DT + at) = lo;
+          const float sc = pow2(-e);
+#pragma unroll
+          for (int c = 0; c < DT / 16; c += 2) {
+            uint2 hi[2], lo[2];
+            split_fp8(w[c], sc, hi[0], lo[0]);
+            split_fp8(w[c + 1], sc, hi[1], lo[1]);
+            const uint32_t at = tile_offset(BM, row, half * (DT / 32) + c / 2);
+            *reinterpret_cast<uint4*>(sQ + at) = make_uint4(hi[0].x, hi[0].y, hi[1].x, hi[1].y);
+            *reinterpret_cast<uint4*>(sQ + BM * DT + at) = make_uint4(lo[0].x, lo[0].y, lo[1].x, lo[1].y);
           }
         }
         sm100::fence_proxy_async_smem();
@@ -816,6 +848,15 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(&p_full[sb]);
       }
+      // the gate, read while the last products run
+      const bool gated = a.gate && live && p.whole;
+      uint4 gw[DT / 16];
+      if (gated) {
+        const bf16* gt = a.gate + p.s * a.g_bs + tok * a.g_ts + hq * a.g_hs + half * (DT / 2);
+#pragma unroll
+        for (int c = 0; c < DT / 16; ++c)
+          gw[c] = half * (DT / 2) + c * 8 < a.D ? *reinterpret_cast<const uint4*>(gt + c * 8) : make_uint4(0, 0, 0, 0);
+      }
       wait_all(o_last, pc & 1);
       sm100::tc_fence_after();
       if (warp_on) {
@@ -823,13 +864,13 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
         // O -> the output (a whole segment) or the workspace
         const float vs = E4M3 ? pow2(ev + 8) : 1.f;
         const float inv = l > 0.f ? vs / l : (l == 0.f ? 0.f : l);
-        // the piece a CTA begins in the middle of its run starts a segment and ends the run
-        const int slot = p.t0 == 0 && walk.end - (p.t1 - p.t0) != U * blockIdx.x / N ? 1 : 0;
+        // a CTA has one part that begins a segment (slot 1) and one that goes on with one (0) at most
+        const int slot = p.t0 == 0;
         const int64_t at = ((int64_t)blockIdx.x * 2 + slot) * rows + row;
         bf16* o = a.out + (((int64_t)p.s * a.T + tok) * a.Hq + hq) * a.D;
-        const bf16* gt = a.gate ? a.gate + p.s * a.g_bs + tok * a.g_ts + hq * a.g_hs : nullptr;
-#pragma unroll 1
-        for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32) {
+#pragma unroll
+        for (int c0 = 0; c0 < DT / 2; c0 += 32) {
+          const int c = half * (DT / 2) + c0;
           float v[32];
           sm100::tmem_ld32(tmem + lane_off + c, v);
           if (!in) continue;
@@ -837,14 +878,15 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
               if (c + i < a.D) {
-                uint32_t w[4], gw[4] = {0, 0, 0, 0};
-                if (gt && live) *reinterpret_cast<uint4*>(gw) = *reinterpret_cast<const uint4*>(gt + c + i);
+                uint32_t w[4];
+                const uint4 g4 = gw[(c0 + i) / 8];
+                const uint32_t gg[4] = {g4.x, g4.y, g4.z, g4.w};
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                   float o0 = v[i + j] * inv, o1 = v[i + j + 1] * inv;
-                  if (gt) {
-                    o0 /= 1.f + __expf(-__uint_as_float(gw[j / 2] << 16));
-                    o1 /= 1.f + __expf(-__uint_as_float(gw[j / 2] & 0xffff0000u));
+                  if (gated) {
+                    o0 *= __fdividef(1.f, 1.f + __expf(-__uint_as_float(gg[j / 2] << 16)));
+                    o1 *= __fdividef(1.f, 1.f + __expf(-__uint_as_float(gg[j / 2] & 0xffff0000u)));
                   }
                   const __nv_bfloat162 h2 = __floats2bfloat162_rn(live ? o0 : 0.f, live ? o1 : 0.f);
                   w[j / 2] = *reinterpret_cast<const uint32_t*>(&h2);
@@ -869,9 +911,8 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
             a.ml[at] = live ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
         }
         if (row == 0 && half == 0 && p.t0 == 0) {  // where the segment's parts are
-          const int64_t first = walk.unit - (p.t1 - p.t0), last = first + p.nt;
-          const int c1 = (int)(((last + 1) * N - 1) / U);
-          a.info[(((int64_t)p.s * a.Hk + p.hk) * a.HB + p.hb) * a.M + p.m] = make_int4(blockIdx.x, c1, slot, 0);
+          const int c1 = p.whole ? (int)blockIdx.x : (int)(((p.last + 1) * N - 1) / U);
+          a.info[(((int64_t)p.s * a.Hk + p.hk) * a.HB + p.hb) * a.M + p.m] = make_int2(blockIdx.x, c1);
         }
       }
       sm100::tc_fence_before();
@@ -1046,49 +1087,62 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
 // One warp per (sequence, token, query head): rows of segments that lie in one CTA are done;
 // the others add their parts in the order of the CTAs.
 __global__ void __launch_bounds__(256) tree_join_kernel(Args a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the tiles are still at work
   const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (i >= (int64_t)a.b * a.T * a.Hq) return;
   const int hq = (int)(i % a.Hq), tok = (int)((i / a.Hq) % a.T), s = (int)(i / ((int64_t)a.Hq * a.T));
   const int hk = hq / a.G, g = hq % a.G, hb = g / a.GT, m = tok / a.TPM;
-  const int4 inf = a.info[(((int64_t)s * a.Hk + hk) * a.HB + hb) * a.M + m];
+  const int2 inf = a.info[(((int64_t)s * a.Hk + hk) * a.HB + hb) * a.M + m];
   if (inf.x == inf.y) return;
-  const int rows = a.GT * a.TPM, row = (tok - m * a.TPM) * a.GT + g - hb * a.GT;
-  float top = -INFINITY;
-  for (int c = inf.x; c <= inf.y; ++c)
-    top = fmaxf(top, a.ml[((int64_t)c * 2 + (c == inf.x ? inf.z : 0)) * rows + row].x);
-  float l = 0.f, o[8] = {};
+  const int rows = a.GT * a.TPM, row = (tok - m * a.TPM) * a.GT + g - hb * a.GT, parts = inf.y - inf.x + 1;
   const bool on = lane * 8 < a.D;
-  for (int c = inf.x; c <= inf.y; ++c) {
-    const int64_t at = ((int64_t)c * 2 + (c == inf.x ? inf.z : 0)) * rows + row;
-    const float2 ml = a.ml[at];
-    const float w = ml.x == -INFINITY ? 0.f : sm100::exp2_approx(ml.x - top);
-    l += w * ml.y;
-    if (on) {
-      const float4 u = *reinterpret_cast<const float4*>(a.part + at * a.D + lane * 8);
-      const float4 v = *reinterpret_cast<const float4*>(a.part + at * a.D + lane * 8 + 4);
-      o[0] += w * u.x, o[1] += w * u.y, o[2] += w * u.z, o[3] += w * u.w;
-      o[4] += w * v.x, o[5] += w * v.y, o[6] += w * v.z, o[7] += w * v.w;
+  const int64_t oi = i * a.D + lane * 8;
+  uint4 gw = make_uint4(0, 0, 0, 0);
+  if (a.gate && on)
+    gw = *reinterpret_cast<const uint4*>(a.gate + s * a.g_bs + tok * a.g_ts + hq * a.g_hs + lane * 8);
+  auto at = [&](int c) -> int64_t { return ((int64_t)(inf.x + c) * 2 + (c == 0)) * rows + row; };
+  float top = -INFINITY, l = 0.f, o[8] = {};
+  for (int c = lane; c < parts; c += 32) top = fmaxf(top, a.ml[at(c)].x);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffff, top, x));
+  for (int c0 = 0; c0 < parts; c0 += 32) {
+    float w = 0.f;  // lane c: weight of part c0 + c
+    if (c0 + lane < parts) {
+      const float2 ml = a.ml[at(c0 + lane)];
+      w = ml.x == -INFINITY ? 0.f : sm100::exp2_approx(ml.x - top);
+      l = fmaf(w, ml.y, l);
+    }
+    const int n = min(32, parts - c0);
+#pragma unroll 4
+    for (int c = 0; c < n; ++c) {
+      const float wc = __shfl_sync(0xffffffff, w, c);
+      if (on) {
+        const float4* p = reinterpret_cast<const float4*>(a.part + at(c0 + c) * a.D + lane * 8);
+        const float4 u = p[0], v = p[1];
+        o[0] = fmaf(wc, u.x, o[0]), o[1] = fmaf(wc, u.y, o[1]), o[2] = fmaf(wc, u.z, o[2]), o[3] = fmaf(wc, u.w, o[3]);
+        o[4] = fmaf(wc, v.x, o[4]), o[5] = fmaf(wc, v.y, o[5]), o[6] = fmaf(wc, v.z, o[6]), o[7] = fmaf(wc, v.w, o[7]);
+      }
     }
   }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffff, l, x);
   const bool live = tok < sequence(a, s, false).cnt;
-  const float inv = live ? 1.f / l : 0.f;
+  const float inv = 1.f / l;
   if (on) {
-    uint32_t gw[4] = {0, 0, 0, 0}, w[4];
-    if (a.gate && live)
-      *reinterpret_cast<uint4*>(gw) =
-          *reinterpret_cast<const uint4*>(a.gate + s * a.g_bs + tok * a.g_ts + hq * a.g_hs + lane * 8);
+    const uint32_t gg[4] = {gw.x, gw.y, gw.z, gw.w};
+    uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
-      float o0 = live ? o[j] * inv : 0.f, o1 = live ? o[j + 1] * inv : 0.f;
+      float o0 = o[j] * inv, o1 = o[j + 1] * inv;
       if (a.gate) {
-        o0 /= 1.f + __expf(-__uint_as_float(gw[j / 2] << 16));
-        o1 /= 1.f + __expf(-__uint_as_float(gw[j / 2] & 0xffff0000u));
+        o0 *= __fdividef(1.f, 1.f + __expf(-__uint_as_float(gg[j / 2] << 16)));
+        o1 *= __fdividef(1.f, 1.f + __expf(-__uint_as_float(gg[j / 2] & 0xffff0000u)));
       }
-      const __nv_bfloat162 h2 = __floats2bfloat162_rn(o0, o1);
+      const __nv_bfloat162 h2 = __floats2bfloat162_rn(live ? o0 : 0.f, live ? o1 : 0.f);
       w[j / 2] = *reinterpret_cast<const uint32_t*>(&h2);
     }
-    *reinterpret_cast<uint4*>(a.out + i * a.D + lane * 8) = *reinterpret_cast<uint4*>(w);
+    *reinterpret_cast<uint4*>(a.out + oi) = *reinterpret_cast<uint4*>(w);
   }
   if (lane == 0)
     a.lse[((int64_t)s * a.Hq + hq) * a.T + tok] = live ? (top + log2f(l)) * 0.6931471805599453f : -INFINITY;
@@ -1216,10 +1270,10 @@ std::vector<at::Tensor> tree_attention(at::Tensor q, at::Tensor k, at::Tensor v,
   // workspace: parts [grid][2][rows][D], their (maximum, sum), and the segments' whereabouts
   const int64_t rows = (int64_t)a.GT * a.TPM, segs = b * a.Hk * a.HB * a.M;
   const int64_t n_part = 2 * grid * rows * D, n_ml = 2 * 2 * grid * rows;
-  at::Tensor ws = at::empty({n_part + ((n_ml + 3) & ~int64_t(3)) + 4 * segs}, lse.options());
+  at::Tensor ws = at::empty({n_part + ((n_ml + 3) & ~int64_t(3)) + 2 * segs}, lse.options());
   a.part = ws.data_ptr<float>();
   a.ml = reinterpret_cast<float2*>(a.part + n_part);
-  a.info = reinterpret_cast<int4*>(a.part + n_part + ((n_ml + 3) & ~int64_t(3)));
+  a.info = reinterpret_cast<int2*>(a.part + n_part + ((n_ml + 3) & ~int64_t(3)));
   // the narrowest tile that holds D; e4m3 operands are at least 128 wide (one swizzle atom)
   if (c.e4m3)
     D <= 128 ? tattn::launch<128, true>(a, grid, c, q, k, v) : tattn::launch<256, true>(a, grid, c, q, k, v);
@@ -1228,8 +1282,16 @@ std::vector<at::Tensor> tree_attention(at::Tensor q, at::Tensor k, at::Tensor v,
   else
     D <= 128 ? tattn::launch<128, false>(a, grid, c, q, k, v) : tattn::launch<256, false>(a, grid, c, q, k, v);
   const int64_t nrows = b * T * Hq;
-  tattn::tree_join_kernel<<<(unsigned)((nrows + 7) / 8), 256, 0, stream()>>>(a);
-  NS_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((nrows + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream();
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  NS_CUDA(cudaLaunchKernelEx(&cfg, tattn::tree_join_kernel, a));
   return {out, lse};
 }
 
