@@ -16,7 +16,8 @@
 //
 // Work is split over the long axis without knowing the lengths on the host: the tiles of
 // all segments (sequence, key head, row tile) are numbered through, and CTA i of N (one per
-// SM) takes tiles [U i / N, U (i+1) / N), so ragged batches and single long sequences load
+// SM) takes units [U i / N, U (i+1) / N) (every segment counts two more for its beginning and
+// end), so ragged batches and single long sequences load
 // every SM alike. A segment that one CTA holds whole is finished there; parts of a segment
 // leave unnormalised O with its reference maximum and sum in a workspace (two parts per CTA
 // at most), and tree_join_kernel adds them up in the order of the CTAs.
@@ -27,12 +28,17 @@
 // e4m3 pages: the codes of K go to the tensor cores as they are (kind::f8f6f4). q, scaled by
 // a power of two per row, is the sum of an e4m3 and an e5m2 matrix: rounding q's 8
 // significant bits to 4 leaves at most 8 units of the last of them, which the 3 of e5m2 hold
-// exactly (elements below 2^-14 of the row's largest are held to 2^-22 of it). V's codes
-// become f16 in shared memory (converter warps; code bits shifted into place, i.e.
-// value * 2^-8, exact) against f16 probabilities (11 bits). The rows' scales stay outside
-// the products: K's multiplies the score, V's the probability, relative to the largest V scale
-// seen so far (when that grows by more than 2^4, O is rescaled like for a growing
-// maximum). The nodes' own rows get scales of the same kind; their K is split like q.
+// exactly (elements below 2^-14 of the row's largest are held to 2^-22 of it). V's codes are
+// multiplied in 8 bits too: P as f16 (11 bits) is the sum of four e5m2 matrices, each the high
+// bytes of what the ones before left. The rows' scales stay outside the products: K's
+// multiplies the score, V's the probability, relative to the largest V scale seen so far
+// (when that grows by more than a factor of 2, O is rescaled like for a growing maximum). The nodes' own
+// K and V are split like q. So no operand is converted on its way to the tensor cores.
+//
+// Measured (32 sequences of 14000 keys, 4 key heads of 256, pages of 64): bf16 390 us at one
+// node (4.71 TB/s) and 428 at 21 (541 TFLOP/s of products, 4.36 TB/s); e4m3 548 and 552 us
+// (1.7 TB/s). bf16 waits for K tiles at 73 % of the copy rate; e4m3 for its issuing and softmax
+// warps, whose work per tile is that of bf16 at half the bytes.
 //
 // Rows of V beyond a sequence's end (stale pages, NaN) are zeroed in shared memory, since
 // 0 * NaN would reach O; masked scores are replaced, not added to. Every mbarrier wait is
@@ -51,12 +57,13 @@ namespace tattn {
 
 constexpr int EXP_BIAS = 127, EXP_MIN = -117, EXP_MAX = 118;
 constexpr int BM = 128, BN = 128;
-constexpr float RESCALE_LOG2 = 8.f;   // the reference maximum may lag by this much
-constexpr int V_RESCALE = 4;          // and the reference V exponent by this much
-constexpr float F16_OFFSET = 3.f;     // f16 probabilities are at most 2^(3 + 8 + 4)
+constexpr float LAG = 8.f;            // the reference maximum may lag by this much (log2); bf16
+constexpr float LAG8 = 6.f;           // e4m3: by this, the reference V exponent by V_LAG, and
+constexpr int V_LAG = 1;              // probabilities are at most 2^(OFFSET8 + 6 + 1) = 2^15, the top of
+constexpr float OFFSET8 = 8.f;        // e5m2, whose smallest step, 2^-16, is 2^-24 of the largest then
 constexpr int SLOT = 16384;           // bytes of one ring slot
 constexpr int SEG_UNITS = 2;          // what beginning and ending a segment costs, in tiles
-constexpr int SOFT_WARPS = 8, CONV_WARPS = 6;
+constexpr int SOFT_WARPS = 8, CONV_WARPS = 2;
 
 struct Args {
   const bf16 *q, *k, *v, *gate;
@@ -238,31 +245,22 @@ struct Ring {
 
 template <int DT, bool E4M3>
 struct Cfg {
-  static constexpr int DA = DT / 64;               // 128-byte swizzle atoms of 16-bit elements along D
-  static constexpr int VK = BN / DA;               // keys in one slot of 16-bit V rows
-  static constexpr int KS = E4M3 ? DT / 128 : DA;  // slots of one K tile
-  static constexpr int RS = E4M3 ? DT / 128 : 0;   // slots of one tile of V codes
-  static constexpr int RK = E4M3 ? BN / (RS + !E4M3) : BN;   // keys in one of them
+  static constexpr int DA = E4M3 ? DT / 128 : DT / 64;  // 128-byte swizzle atoms along D: ring slots of a K or V tile
+  static constexpr int AC = E4M3 ? 128 : 64;       // channels of one
+  static constexpr int VK = BN / DA;               // keys in one slot of V
+  static constexpr int KQ = E4M3 ? 32 : 16;        // keys of one product with P
+  static constexpr int PP = E4M3 ? 4 : 2;          // matrices whose sum is P
   static constexpr int Q_BYTES = BM * DT * 2;      // bf16, or the two 8-bit matrices
-  // Ring sizes (slots). bf16: one ring, K and V in the order of the products. e4m3: K codes,
-  // V codes, f16 V.
-  static constexpr int NK = E4M3 ? 4 : (DT == 256 ? 9 : 11);
-  static constexpr int NR = E4M3 ? (DT == 256 ? 2 : 3) : 0;
-  static constexpr int NV = E4M3 ? (DT == 256 ? 3 : 4) : 0;
-  static constexpr int PP = E4M3 ? 1 : 2;          // matrices whose sum is P
+  static constexpr int NK = DT == 256 ? 9 : 11;    // ring slots, K and V in the order of the products
   static constexpr int XCH = 2 * 2 * 2 * BM * 4;   // maxima and sums exchanged by a row's two threads
-  // e4m3 scales of FAC tiles: exponent bytes, K and V factors, largest V exponent. Buffer n % FAC
-  // is written again for tile n + FAC once that tile has its KS ring slots, the last of which
-  // held tile n + 2 or a later one (NK <= KS (FAC - 2)); and S of tile n + 2 is only issued
-  // after P of tile n was formed.
-  static constexpr int FAC = KS == 2 ? 4 : 8;
-  static constexpr int FACS = E4M3 ? FAC * (2 * BN + 2 * BN * 4 + 16) : 0;
-  static constexpr int SMEM = Q_BYTES + (NK + NR + NV) * SLOT + FACS + XCH + 128 + 512 + 1024;
+  // e4m3 scales of FAC tiles: exponent bytes, K and V factors, largest V exponent
+  static constexpr int FAC = 4;
+  static constexpr int FACS = E4M3 ? FAC * (2 * BN + 2 * BN * 2 + 16) + MAX_NODES * 4 : 0;
+  static constexpr int SMEM = Q_BYTES + NK * SLOT + FACS + XCH + 128 + 512 + 1024;
   static constexpr int S_COL = DT;
-  static constexpr int TMEM_COLS = DT + 2 * BN <= 256 ? 256 : 512;
+  static constexpr int TMEM_COLS = 512;            // DT + 2 BN, a power of two
   static constexpr int THREADS = 32 * (2 + SOFT_WARPS + (E4M3 ? CONV_WARPS : 0));
   static_assert(SMEM <= 232448, "shared memory");
-  static_assert(!E4M3 || NK <= KS * (FAC - 2), "scale buffers");
 };
 
 // Tiles of a piece in the order of the products: S0, (S1, PV0), (S2, PV1), .., PV(n-1).
@@ -291,16 +289,6 @@ __device__ __forceinline__ uint32_t finite_top(uint4 w) {  // largest finite mag
   return top;
 }
 
-__device__ __forceinline__ uint4 scale_to_f16(uint4 w, float s) {  // 8 bf16
-  uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2 h = __floats2half2_rn(__uint_as_float(x[i] << 16) * s, __uint_as_float(x[i] & 0xffff0000u) * s);
-    x[i] = *reinterpret_cast<const uint32_t*>(&h);
-  }
-  return make_uint4(x[0], x[1], x[2], x[3]);
-}
-
 // 8 bf16 times s as the sum of e4m3 and e5m2
 __device__ __forceinline__ void split_fp8(uint4 w, float s, uint2& hi, uint2& lo) {
   const uint32_t x[4] = {w.x, w.y, w.z, w.w};
@@ -318,15 +306,17 @@ __device__ __forceinline__ void split_fp8(uint4 w, float s, uint2& hi, uint2& lo
   lo = make_uint2(l[0], l[1]);
 }
 
-// 4 e4m3 codes -> 4 f16 of value * 2^-8: exponent and mantissa bits shifted into place (both
-// formats count subnormals the same way). NaN codes become 1.875 here.
-__device__ __forceinline__ uint2 codes_to_f16(uint32_t w) {
-  const uint32_t a = __byte_perm(w, 0, 0x1404), b = __byte_perm(w, 0, 0x3424);
-  return make_uint2((a & 0x80008000u) | ((a & 0x7f007f00u) >> 1), (b & 0x80008000u) | ((b & 0x7f007f00u) >> 1));
+__device__ __forceinline__ uint4 lds4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
 }
 
-__device__ __forceinline__ uint32_t nan_codes(uint32_t w) {  // non-zero if one of 4 codes is NaN
-  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+// what e5m2 leaves of two f16
+__device__ __forceinline__ uint32_t high_bytes_off(uint32_t w) {
+  const uint32_t top = w & 0xff00ff00u;
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&top));
+  return *reinterpret_cast<const uint32_t*>(&d);
 }
 
 // byte offset of 16-byte chunk c of row r in a K-major 128-byte-swizzled tile of `rows` rows
@@ -340,37 +330,33 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
                      const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tkp,
                      const __grid_constant__ CUtensorMap tvp, Args a) {
   using C = Cfg<DT, E4M3>;
-  constexpr int DA = C::DA, VK = C::VK, KS = C::KS, NK = C::NK, NR = C::NR, NV = C::NV, FAC = C::FAC;
+  constexpr int DA = C::DA, VK = C::VK, NK = C::NK, FAC = C::FAC;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sQ = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sK = sQ + C::Q_BYTES;      // [NK] (bf16: K and V)
-  uint8_t* sRaw = sK + NK * SLOT;     // [NR] codes of V
-  uint8_t* sV = E4M3 ? sRaw + NR * SLOT : sK;
-  float* kfac = reinterpret_cast<float*>(sK + (NK + NR + NV) * SLOT);  // [FAC][BN] 2^e of K rows
-  float* vfac = kfac + (E4M3 ? FAC * BN : 0);                          // [FAC][BN] 2^(e - emax) of V rows
-  int* vmax = reinterpret_cast<int*>(vfac + (E4M3 ? FAC * BN : 0));    // [FAC][4] emax of each tile
-  uint8_t* sExp = reinterpret_cast<uint8_t*>(vmax + (E4M3 ? FAC * 4 : 0));  // [FAC][2][BN] exponent bytes
-  float* xmax = reinterpret_cast<float*>(sExp + (E4M3 ? FAC * 2 * BN : 0));  // [2][2][BM]
-  float* xsum = xmax + 2 * 2 * BM;                                           // [2][2][BM]
-  int* page_rows = reinterpret_cast<int*>(xsum + 2 * 2 * BM);                // [4][8] of the producer
+  uint8_t* sKV = sQ + C::Q_BYTES;                                        // [NK]
+  bf16* kfac = reinterpret_cast<bf16*>(sKV + NK * SLOT);                 // [FAC][BN] 2^e of K rows
+  __half* vfac = reinterpret_cast<__half*>(kfac + (E4M3 ? FAC * BN : 0));  // [FAC][BN] 2^(e - emax) of V rows
+  int* vmax = reinterpret_cast<int*>(vfac + (E4M3 ? FAC * BN : 0));      // [FAC][4] emax of each tile
+  int* vexp = vmax + (E4M3 ? FAC * 4 : 0);                               // [MAX_NODES] exponents of the nodes' V
+  uint8_t* sExp = reinterpret_cast<uint8_t*>(vexp + (E4M3 ? MAX_NODES : 0));  // [FAC][2][BN] exponent bytes
+  float* xmax = reinterpret_cast<float*>(sExp + (E4M3 ? FAC * 2 * BN : 0));   // [2][2][BM]
+  float* xsum = xmax + 2 * 2 * BM;                                            // [2][2][BM]
+  int* page_rows = reinterpret_cast<int*>(xsum + 2 * 2 * BM);                 // [4][8] of the producer
   uint64_t* bars = reinterpret_cast<uint64_t*>(page_rows + 32);
-  uint64_t* k_full = bars;           // [NK]
-  uint64_t* k_empty = k_full + NK;   // [NK]
-  uint64_t* r_full = k_empty + NK;   // [NR]
-  uint64_t* r_empty = r_full + NR;   // [NR]
-  uint64_t* v_full = E4M3 ? r_empty + NR : k_full;   // [NV]
-  uint64_t* v_empty = E4M3 ? v_full + NV : k_empty;  // [NV]
-  uint64_t* e_full = r_empty + NR + 2 * NV;          // [FAC] exponent bytes landed
-  uint64_t* f_full = e_full + (E4M3 ? FAC : 0);      // [FAC] factors ready
-  uint64_t* s_full = f_full + (E4M3 ? FAC : 0);      // [2]
-  uint64_t* p_full = s_full + 2;                     // [2]
+  uint64_t* full = bars;             // [NK]
+  uint64_t* empty = full + NK;       // [NK]
+  uint64_t* e_full = empty + NK;     // [FAC] exponent bytes landed (e4m3)
+  uint64_t* f_full = e_full + FAC;   // [FAC] factors ready
+  uint64_t* f_free = f_full + FAC;   // [FAC] factors read
+  uint64_t* s_full = f_free + FAC;   // [2]
+  uint64_t* p_full = s_full + 2;     // [2]
   uint64_t* q_full = p_full + 2;
   uint64_t* q_empty = q_full + 1;
   uint64_t* o_done = q_empty + 1;  // one completion per PV (rescales wait for the previous one)
   uint64_t* o_last = o_done + 1;   // one per piece, after its last PV
   uint64_t* o_free = o_last + 1;   // one per piece, O has been read
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 1);
-  static_assert(2 * (NK + NR + NV + FAC) + 9 + 1 <= 64, "barrier area");
+  static_assert(2 * NK + 3 * FAC + 9 + 1 <= 64, "barrier area");
 
   // the join may be set up now; it waits for this kernel's end
   asm volatile("griddepcontrol.launch_dependents;");
@@ -381,10 +367,12 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
   if (walk.unit >= walk.end) return;
 
   if (warp == 0 && lane == 0) {
-    for (int i = 0; i < NK; ++i) sm100::mbar_init(&k_full[i], 1), sm100::mbar_init(&k_empty[i], 1);
-    for (int i = 0; i < NR; ++i) sm100::mbar_init(&r_full[i], 1), sm100::mbar_init(&r_empty[i], CONV_WARPS);
-    for (int i = 0; i < NV; ++i) sm100::mbar_init(&v_full[i], CONV_WARPS), sm100::mbar_init(&v_empty[i], 1);
-    for (int i = 0; i < (E4M3 ? FAC : 0); ++i) sm100::mbar_init(&e_full[i], 1), sm100::mbar_init(&f_full[i], 1);
+    for (int i = 0; i < NK; ++i) sm100::mbar_init(&full[i], 1), sm100::mbar_init(&empty[i], 1);
+    for (int i = 0; i < FAC; ++i) {
+      sm100::mbar_init(&e_full[i], 1);
+      sm100::mbar_init(&f_full[i], 1);
+      sm100::mbar_init(&f_free[i], SOFT_WARPS);
+    }
     for (int i = 0; i < 2; ++i) sm100::mbar_init(&s_full[i], 1), sm100::mbar_init(&p_full[i], SOFT_WARPS);
     sm100::mbar_init(q_full, E4M3 ? SOFT_WARPS : 1);
     sm100::mbar_init(q_empty, 1);
@@ -408,11 +396,8 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
   if (warp == 0) {
     // ---------------------------------------------------------- TMA producer
     // The whole warp waits; one elected lane issues (ptxas then keeps the operands uniform).
-    constexpr int VR = E4M3 ? C::RK : VK;  // keys of one slot of the pages' V rows
-    constexpr int VA = E4M3 ? DT / 64 : DA;
-    constexpr int ROW = E4M3 ? 64 : 128;   // bytes of such a row in one column block
-    const int kb = min(a.page, BN), vb = min(a.page, VR);  // rows that one copy brings
-    Ring kr, rr;
+    const int kb = min(a.page, BN), vb = min(a.page, VK);  // rows that one copy brings
+    Ring r;
     int n = 0, pc = 0;
     bool ok = true;
     // pool rows of 16 keys each (lane l: keys 16 l ..) of tile t, kept in shared memory for the
@@ -446,71 +431,68 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
         const int keys = p.keys(t);
         const bool own = t == p.nt;
         const int* rows = page_rows + (t & 3) * 8;
-        if (!pv) {
+        if (E4M3 && own) {  // the converters fill these
+          for (int j = 0; j < (pv && keys == 0 ? 0 : DA); ++j) r.step(NK);
+          n += !pv;
+        } else if (!pv) {
           const int runs = (keys + kb - 1) / kb;
           if (t + 1 < p.t1) look_up(t + 1);
-          if (E4M3 && own) {  // the converters fill these
-            for (int j = 0; j < KS; ++j) kr.step(NK);
-          } else {
 #pragma unroll 1
-            for (int j = 0; j < KS; ++j) {
-              ok = ok && wait(&k_empty[kr.st], kr.ph ^ 1, a.err);
-              if (sm100::elect_one() && ok) {
-                uint64_t* fb = &k_full[kr.st];
-                uint8_t* d = sK + kr.st * SLOT;
-                if (own) {
-                  sm100::mbar_expect_tx(fb, a.T * 128);
-                  sm100::tma_load_4d(d, &tk, fb, 64 * j, p.hk, 0, p.s);
-                } else {
-                  sm100::mbar_expect_tx(fb, runs * kb * 128);
-                  for (int r = 0; r < runs; ++r)
-                    sm100::tma_load_2d(d + r * kb * 128, &tkp, fb, (E4M3 ? 128 : 64) * j, rows[r * kb / 16]);
-                }
+          for (int j = 0; j < DA; ++j) {
+            ok = ok && wait(&empty[r.st], r.ph ^ 1, a.err);
+            if (sm100::elect_one() && ok) {
+              uint64_t* fb = &full[r.st];
+              uint8_t* d = sKV + r.st * SLOT;
+              if (own) {
+                sm100::mbar_expect_tx(fb, a.T * 128);
+                sm100::tma_load_4d(d, &tk, fb, 64 * j, p.hk, 0, p.s);
+              } else {
+                sm100::mbar_expect_tx(fb, runs * kb * 128);
+                for (int x = 0; x < runs; ++x)
+                  sm100::tma_load_2d(d + x * kb * 128, &tkp, fb, C::AC * j, rows[x * kb / 16]);
               }
-              __syncwarp();
-              kr.step(NK);
             }
+            __syncwarp();
+            r.step(NK);
           }
           if constexpr (E4M3) {
-            if (!own) {
-              if (sm100::elect_one() && ok) {
-                uint64_t* eb = &e_full[n % FAC];
-                sm100::mbar_expect_tx(eb, runs * kb * 2);
-                for (int r = 0; r < runs; ++r) {
-                  sm100::bulk_load(sExp + (n % FAC) * 2 * BN + r * kb, a.ke + rows[r * kb / 16], kb, eb);
-                  sm100::bulk_load(sExp + ((n % FAC) * 2 + 1) * BN + r * kb, a.ve + rows[r * kb / 16], kb, eb);
-                }
+            uint64_t* eb = &e_full[n % FAC];
+            if (n >= FAC) ok = ok && wait(&f_free[n % FAC], (n / FAC - 1) & 1, a.err);
+            if (sm100::elect_one() && ok) {
+              sm100::mbar_expect_tx(eb, runs * kb * 2);
+              for (int x = 0; x < runs; ++x) {
+                sm100::bulk_load(sExp + (n % FAC) * 2 * BN + x * kb, a.ke + rows[x * kb / 16], kb, eb);
+                sm100::bulk_load(sExp + ((n % FAC) * 2 + 1) * BN + x * kb, a.ve + rows[x * kb / 16], kb, eb);
               }
-              __syncwarp();
             }
+            __syncwarp();
             ++n;
           }
-        } else if (!E4M3 || !own) {
-          Ring& r = E4M3 ? rr : kr;
+        } else {
 #pragma unroll 1
-          for (int i = 0; i * VR < keys; ++i) {
-            ok = ok && wait(E4M3 ? &r_empty[r.st] : &k_empty[r.st], r.ph ^ 1, a.err);
+          for (int i = 0; i * VK < keys; ++i) {
+            ok = ok && wait(&empty[r.st], r.ph ^ 1, a.err);
             if (sm100::elect_one() && ok) {
-              uint64_t* fb = E4M3 ? &r_full[r.st] : &k_full[r.st];
-              uint8_t* d = (E4M3 ? sRaw : sK) + r.st * SLOT;
+              uint64_t* fb = &full[r.st];
+              uint8_t* d = sKV + r.st * SLOT;
               if (own) {
                 sm100::mbar_expect_tx(fb, DA * min(a.T, VK) * 128);
 #pragma unroll
                 for (int j = 0; j < DA; ++j)
                   sm100::tma_load_4d(d + j * (VK * 128), &tv, fb, 64 * j, p.hk, i * VK, p.s);
               } else {
-                const int runs = (min(VR, keys - i * VR) + vb - 1) / vb;
-                sm100::mbar_expect_tx(fb, VA * runs * vb * ROW);
+                const int runs = (min(VK, keys - i * VK) + vb - 1) / vb;
+                sm100::mbar_expect_tx(fb, DA * runs * vb * 128);
                 for (int u = 0; u < runs; ++u) {
-                  const int row = rows[(i * VR + u * vb) / 16];
+                  const int row = rows[(i * VK + u * vb) / 16];
 #pragma unroll
-                  for (int j = 0; j < VA; ++j)
-                    sm100::tma_load_2d(d + j * (VR * ROW) + u * vb * ROW, &tvp, fb, 64 * j, row);
+                  for (int j = 0; j < DA; ++j)
+                    sm100::tma_load_2d(d + j * (VK * 128) + u * vb * 128, &tvp, fb, C::AC * j, row);
                 }
               }
             }
             __syncwarp();
-            r.step(E4M3 ? NR : NK);
+            r.step(NK);
           }
         }
       });
@@ -518,12 +500,8 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
     // drain: every issued copy has landed before the CTA may exit
     if (!E4M3 && pc > 0) wait(q_full, (pc - 1) & 1, a.err);
     for (int i = 0; i < NK; ++i) {  // slots that were never armed count as empty
-      wait(&k_empty[kr.st], kr.ph ^ 1, a.err);
-      kr.step(NK);
-    }
-    for (int i = 0; i < NR; ++i) {
-      wait(&r_empty[rr.st], rr.ph ^ 1, a.err);
-      rr.step(NR);
+      wait(&empty[r.st], r.ph ^ 1, a.err);
+      r.step(NK);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
@@ -531,11 +509,13 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
     // waits (the whole warp) and products (one elected lane: ptxas then keeps the operands
     // uniform, without a loop over lanes around each); descriptors are a constant plus offsets
     // in 16-byte units.
-    constexpr uint32_t idesc_o = E4M3 ? sm100::idesc_f16(BM, DT, false, true) : sm100::idesc_bf16(BM, DT, false, true);
+    constexpr uint32_t E5M2_A = 1u << 7, E5M2_B = 1u << 10;  // kind::f8f6f4: e4m3 otherwise
+    constexpr uint32_t idesc_o =
+        E4M3 ? sm100::idesc_e4m3(BM, DT, false, true) | E5M2_A : sm100::idesc_bf16(BM, DT, false, true);
     const uint64_t dq = sm100::smem_desc_sw128(sm100::smem_u32(sQ), 0, 1024);
-    const uint64_t dk = sm100::smem_desc_sw128(sm100::smem_u32(sK), 0, 1024);
-    const uint64_t dv = sm100::smem_desc_sw128(sm100::smem_u32(sV), VK * 128, 1024);
-    Ring kr, vr;
+    const uint64_t dk = sm100::smem_desc_sw128(sm100::smem_u32(sKV), 0, 1024);
+    const uint64_t dv = sm100::smem_desc_sw128(sm100::smem_u32(sKV), VK * 128, 1024);
+    Ring r;
     int n = 0, ns = 0, pc = 0;  // PV tile, S tile, piece
     bool ok = true;
     while (walk.next(a, p)) {
@@ -543,98 +523,123 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
       product_order(p.t0, p.t1, [&](int t, bool pv) {
         const int keys = p.keys(t);
         const bool own = t == p.nt;
+        // the slots of the second matrix of the nodes' rows (e4m3 form)
+        const uint64_t lo_off = DT == 256 ? (uint64_t)((r.st + 1) % NK * (SLOT / 16)) : r.st * (SLOT / 16) + MAX_NODES * 8;
         if (!pv) {
           const uint32_t cols = max(16, (keys + 15) & ~15);
-          const uint32_t idesc = sm100::idesc_bf16(BM, 16, false, false) - (2u << 17) + ((cols >> 3) << 17);
-          const uint32_t idesc8 = idesc & ~((1u << 7) | (1u << 10));  // e4m3 x e4m3; bits 7 / 10: e5m2
+          const uint32_t idesc = (E4M3 ? sm100::idesc_e4m3(BM, 0, false, false) : sm100::idesc_bf16(BM, 0, false, false)) +
+                                 ((cols >> 3) << 17);
           const uint32_t d = tmem + C::S_COL + (ns & 1) * BN;
           // the buffer's last reader, and every product before it, is done
           if (n > 0) ok = ok && wait(o_done, (n - 1) & 1, a.err);
-          if (E4M3 && own) {  // (Q hi + Q lo) (K hi + K lo), the two K matrices of 64 rows one after the other
-            const Ring k0 = kr;
-            for (int j = 0; j < KS; ++j) {
-              ok = ok && wait(&k_full[kr.st], kr.ph, a.err);
-              kr.step(NK);
+          if (E4M3 && own) {  // (Q hi + Q lo) (K hi + K lo), K matrices of 64 rows
+            const Ring k0 = r;
+            for (int j = 0; j < DA; ++j) {
+              ok = ok && wait(&full[r.st], r.ph, a.err);
+              r.step(NK);
             }
             sm100::tc_fence_after();
             if (sm100::elect_one() && ok) {
-              const uint64_t hi = dk + k0.st * (SLOT / 16);
-              const uint64_t lo = DT == 256 ? dk + (k0.st + 1) % NK * (SLOT / 16) : hi + MAX_NODES * 8;
+              const uint64_t hi = dk + k0.st * (SLOT / 16), lo = dk + lo_off;
 #pragma unroll 1
               for (int x = 0; x < 4; ++x) {
 #pragma unroll
                 for (int kk = 0; kk < DT / 32; ++kk)
                   sm100::mma_f8(d, dq + (x & 1) * (BM * DT / 16) + (kk >> 2) * (BM * 8) + (kk & 3) * 2,
                                 (x >> 1 ? lo : hi) + (kk >> 2) * (MAX_NODES * 8) + (kk & 3) * 2,
-                                idesc8 | (x & 1) << 7 | (x >> 1) << 10, x + kk > 0 ? 1u : 0u);
+                                idesc | (x & 1) * E5M2_A | (x >> 1) * E5M2_B, x + kk > 0 ? 1u : 0u);
               }
-              sm100::mma_commit(&k_empty[k0.st]);
-              if (KS == 2) sm100::mma_commit(&k_empty[(k0.st + 1) % NK]);
+              sm100::mma_commit(&empty[k0.st]);
+              if (DA == 2) sm100::mma_commit(&empty[(k0.st + 1) % NK]);
+              sm100::mma_commit(&s_full[ns & 1]);
             }
           } else {
 #pragma unroll
-            for (int j = 0; j < KS; ++j) {
-              ok = ok && wait(&k_full[kr.st], kr.ph, a.err);
+            for (int j = 0; j < DA; ++j) {
+              ok = ok && wait(&full[r.st], r.ph, a.err);
               sm100::tc_fence_after();
               if (sm100::elect_one() && ok) {
-                const uint64_t kd = dk + kr.st * (SLOT / 16);
+                const uint64_t kd = dk + r.st * (SLOT / 16);
                 if constexpr (E4M3) {
 #pragma unroll
                   for (int x = 0; x < 2; ++x)
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                      sm100::mma_f8(d, dq + (x * (BM * DT / 16) + j * (BM * 8) + kk * 2), kd + kk * 2, idesc8 | x << 7,
-                                    j + x + kk > 0 ? 1u : 0u);
+                      sm100::mma_f8(d, dq + (x * (BM * DT / 16) + j * (BM * 8) + kk * 2), kd + kk * 2,
+                                    idesc | x * E5M2_A, j + x + kk > 0 ? 1u : 0u);
                 } else {
 #pragma unroll
                   for (int kk = 0; kk < 4; ++kk)
                     sm100::mma_bf16(d, dq + (j * (BM * 8) + kk * 2), kd + kk * 2, idesc, j + kk > 0 ? 1u : 0u);
                 }
-                sm100::mma_commit(&k_empty[kr.st]);
-                if (j == KS - 1) sm100::mma_commit(&s_full[ns & 1]);
+                sm100::mma_commit(&empty[r.st]);
+                if (j == DA - 1) sm100::mma_commit(&s_full[ns & 1]);
               }
-              kr.step(NK);
+              r.step(NK);
             }
           }
-          if (((E4M3 && own) || (!E4M3 && t == p.t1 - 1)) && sm100::elect_one() && ok) {
-            if (E4M3 && own) sm100::mma_commit(&s_full[ns & 1]);
-            if (!E4M3) sm100::mma_commit(q_empty);
-          }
+          if (!E4M3 && t == p.t1 - 1 && sm100::elect_one() && ok) sm100::mma_commit(q_empty);
           ++ns;
         } else {
           const int pb = n & 1;
           const uint32_t ps = tmem + C::S_COL + pb * BN;
-          Ring& r = E4M3 ? vr : kr;
           ok = ok && wait(&p_full[pb], (n >> 1) & 1, a.err);
           if (t == p.t0 && pc > 0) ok = ok && wait(o_free, (pc - 1) & 1, a.err);
-          auto product = [&](int k16, uint64_t bd) {  // P of 16 keys: 8 columns of its half's 64
+          // P of KQ keys: 8 columns of each of its matrices, 32 keys in the columns of their scores
+          auto product = [&](int kq, uint64_t bd, uint32_t idesc, bool first) {
+            constexpr int H = 32 / C::KQ;  // products of 32 keys
 #pragma unroll
-            for (int x = 0; x < C::PP; ++x)
-              sm100::mma_f16_ts(tmem, ps + (k16 >> 2) * 64 + x * 32 + (k16 & 3) * 8, bd, idesc_o,
-                                (t > p.t0 || k16 + x > 0) ? 1u : 0u);
+            for (int x = 0; x < C::PP; ++x) {
+              const uint32_t ad = ps + kq / H * 32 + x * (H * 8) + kq % H * 8;
+              const uint32_t acc = (first && x == 0) ? 0u : 1u;
+              if constexpr (E4M3)
+                sm100::mma_f8_ts(tmem, ad, bd, idesc, acc);
+              else
+                sm100::mma_f16_ts(tmem, ad, bd, idesc, acc);
+            }
           };
-          if (keys == BN) {
+          constexpr int KS = VK / C::KQ;  // products of one slot
+          if (E4M3 && own) {
+            if (keys > 0) {
+              const Ring v0 = r;
+              for (int j = 0; j < DA; ++j) {
+                ok = ok && wait(&full[r.st], r.ph, a.err);
+                r.step(NK);
+              }
+              sm100::tc_fence_after();
+              if (sm100::elect_one() && ok) {
+#pragma unroll 1
+                for (int kk = 0; kk * C::KQ < keys; ++kk) {
+                  product(kk, dv + v0.st * (SLOT / 16) + kk * (C::KQ * 8), idesc_o, t == p.t0 && kk == 0);
+                  product(kk, dv + lo_off + kk * (C::KQ * 8), idesc_o | E5M2_B, false);
+                }
+                sm100::mma_commit(&empty[v0.st]);
+                if (DA == 2) sm100::mma_commit(&empty[(v0.st + 1) % NK]);
+              }
+            }
+            if (sm100::elect_one() && ok) sm100::mma_commit(o_done);
+          } else if (keys == BN) {
 #pragma unroll
             for (int i = 0; i < DA; ++i) {
-              ok = ok && wait(&v_full[r.st], r.ph, a.err);
+              ok = ok && wait(&full[r.st], r.ph, a.err);
               sm100::tc_fence_after();
               if (sm100::elect_one() && ok) {
 #pragma unroll
-                for (int kk = 0; kk < VK / 16; ++kk)
-                  product(i * (VK / 16) + kk, dv + r.st * (SLOT / 16) + kk * 128);
-                sm100::mma_commit(&v_empty[r.st]);
+                for (int kk = 0; kk < KS; ++kk)
+                  product(i * KS + kk, dv + r.st * (SLOT / 16) + kk * (C::KQ * 8), idesc_o, t == p.t0 && i + kk == 0);
+                sm100::mma_commit(&empty[r.st]);
                 if (i == DA - 1) sm100::mma_commit(o_done);
               }
-              r.step(E4M3 ? NV : NK);
+              r.step(NK);
             }
           } else {
 #pragma unroll 1
             for (int i = 0; i * VK < keys; ++i) {
-              const int live = min(VK, keys - i * VK);
-              ok = ok && wait(&v_full[r.st], r.ph, a.err);
-              if (!E4M3 && (live & 15)) {  // rows beyond the end, up to the next product's edge
-                for (int x = lane; x < (16 - (live & 15)) * 8 * DA; x += 32)
-                  *reinterpret_cast<uint4*>(sV + r.st * SLOT + tile_offset(VK, live + x / (8 * DA), x % (8 * DA))) =
+              const int live = min(VK, keys - i * VK), dead = -live & (C::KQ - 1);
+              ok = ok && wait(&full[r.st], r.ph, a.err);
+              if (dead) {  // rows beyond the end, up to the next product's edge
+                for (int x = lane; x < dead * 8 * DA; x += 32)
+                  *reinterpret_cast<uint4*>(sKV + r.st * SLOT + tile_offset(VK, live + x / (8 * DA), x % (8 * DA))) =
                       make_uint4(0, 0, 0, 0);
                 sm100::fence_proxy_async_smem();
                 __syncwarp();
@@ -642,11 +647,11 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
               sm100::tc_fence_after();
               if (sm100::elect_one() && ok) {
 #pragma unroll 1
-                for (int kk = 0; kk * 16 < live; ++kk)
-                  product(i * (VK / 16) + kk, dv + r.st * (SLOT / 16) + kk * 128);
-                sm100::mma_commit(&v_empty[r.st]);
+                for (int kk = 0; kk * C::KQ < live; ++kk)
+                  product(i * KS + kk, dv + r.st * (SLOT / 16) + kk * (C::KQ * 8), idesc_o, t == p.t0 && i + kk == 0);
+                sm100::mma_commit(&empty[r.st]);
               }
-              r.step(E4M3 ? NV : NK);
+              r.step(NK);
             }
             if (sm100::elect_one() && ok) sm100::mma_commit(o_done);
           }
@@ -684,30 +689,41 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
       float rs = a.scale_log2;  // multiplies the products of this row
       if constexpr (E4M3) {
         // q row -> e4m3 and e5m2 rows with a power-of-two scale (the previous piece's products are
-        // complete: this thread has seen all of its scores); this thread's half in one round of loads
+        // complete: this thread has seen all of its scores); this thread's half
         if (warp_on) {
-          uint4 w[DT / 16];
+          constexpr int QC = DT / 16;  // 16-byte chunks of a half, 8 at a time (registers)
           const bf16* q = a.q + p.s * a.q_bs + tok * a.q_ts + hq * a.q_hs + half * (DT / 2);
+          auto load = [&](int c0, uint4 (&w)[8]) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              w[c] = make_uint4(0, 0, 0, 0);
+              if (live && half * (DT / 2) + (c0 + c) * 8 < a.D) w[c] = *reinterpret_cast<const uint4*>(q + (c0 + c) * 8);
+            }
+          };
           uint32_t top = 0;
+          uint4 w[8];
+#pragma unroll 1
+          for (int c0 = 0; c0 < QC; c0 += 8) {
+            load(c0, w);
 #pragma unroll
-          for (int c = 0; c < DT / 16; ++c) {
-            w[c] = make_uint4(0, 0, 0, 0);
-            if (live && half * (DT / 2) + c * 8 < a.D) w[c] = *reinterpret_cast<const uint4*>(q + c * 8);
+            for (int c = 0; c < 8; ++c) top = max(top, finite_top(w[c]));
           }
-#pragma unroll
-          for (int c = 0; c < DT / 16; ++c) top = max(top, finite_top(w[c]));
           top = max(top, __float_as_uint(exchange(xsum + (pc & 1 ^ 1) * 2 * BM, __uint_as_float(top))));
           const int e = row_exponent(top, 7);
           rs *= pow2(e);
           const float sc = pow2(-e);
+#pragma unroll 1
+          for (int c0 = 0; c0 < QC; c0 += 8) {
+            if (QC > 8) load(c0, w);
 #pragma unroll
-          for (int c = 0; c < DT / 16; c += 2) {
-            uint2 hi[2], lo[2];
-            split_fp8(w[c], sc, hi[0], lo[0]);
-            split_fp8(w[c + 1], sc, hi[1], lo[1]);
-            const uint32_t at = tile_offset(BM, row, half * (DT / 32) + c / 2);
-            *reinterpret_cast<uint4*>(sQ + at) = make_uint4(hi[0].x, hi[0].y, hi[1].x, hi[1].y);
-            *reinterpret_cast<uint4*>(sQ + BM * DT + at) = make_uint4(lo[0].x, lo[0].y, lo[1].x, lo[1].y);
+            for (int c = 0; c < 8; c += 2) {
+              uint2 hi[2], lo[2];
+              split_fp8(w[c], sc, hi[0], lo[0]);
+              split_fp8(w[c + 1], sc, hi[1], lo[1]);
+              const uint32_t at = tile_offset(BM, row, half * (DT / 32) + (c0 + c) / 2);
+              *reinterpret_cast<uint4*>(sQ + at) = make_uint4(hi[0].x, hi[0].y, hi[1].x, hi[1].y);
+              *reinterpret_cast<uint4*>(sQ + BM * DT + at) = make_uint4(lo[0].x, lo[0].y, lo[1].x, lo[1].y);
+            }
           }
         }
         sm100::fence_proxy_async_smem();
@@ -738,16 +754,23 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
         float alpha_o = 1.f;
         bool grow = false;
         const uint32_t scol = tmem + lane_off + C::S_COL + sb * BN + half * 64;
-        const float* kf = kfac + (n % FAC) * BN + half * 64;
-        const float* vf = vfac + (n % FAC) * BN + half * 64;
+        const uint32_t kf = sm100::smem_u32(kfac + (n % FAC) * BN + half * 64);
+        const uint32_t vf = sm100::smem_u32(vfac + (n % FAC) * BN + half * 64);
         // 32 scores: read, K's scale (e4m3), mask
         auto scores = [&](int c0, float (&x)[32]) {
           sm100::tmem_ld32(scol + c0, x);
           if constexpr (E4M3) {
+            uint4 f[4];
 #pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(kf + c0 + c);
-              x[c] *= f.x, x[c + 1] *= f.y, x[c + 2] *= f.z, x[c + 3] *= f.w;
+            for (int c = 0; c < 4; ++c) f[c] = lds4(kf + (c0 + c * 8) * 2);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t w[4] = {f[c].x, f[c].y, f[c].z, f[c].w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                x[c * 8 + 2 * i] *= __uint_as_float(w[i] << 16);
+                x[c * 8 + 2 * i + 1] *= __uint_as_float(w[i] & 0xffff0000u);
+              }
             }
           }
           const uint32_t mk = (uint32_t)(mask >> c0);
@@ -757,42 +780,42 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
               if (!(mk & (1u << c))) x[c] = -INFINITY;
           }
         };
-        auto largest = [&](const float (&x)[32]) -> float {
-          float mx[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = x[i];
-#pragma unroll
-          for (int c = 4; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
-          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        };
-        float x[E4M3 ? 1 : 2][32];  // the e4m3 form has fewer registers and reads them again
-        if (warp_on) {
-          scores(0, x[0]);
-          float mt = largest(x[0]);
-          scores(32, x[C::PP - 1]);
-          mt = fmaxf(mt, largest(x[C::PP - 1]));
-          mt = fmaxf(mt, exchange(xmax + sb * 2 * BM, mt));
-          const float top = mt * rs - (E4M3 ? F16_OFFSET : 0.f);
-          if (live && top > m + RESCALE_LOG2) {
-            alpha_o = sm100::exp2_approx(m - top);  // 0 on the first tile
-            l *= alpha_o;
-            m = top;
-            grow = true;
-          }
-        }
-        float ref = m == -INFINITY ? 0.f : m, back = 1.f;
+        float back = 1.f, shift = 0.f;  // this tile's V scale relative to the reference (e4m3)
         if constexpr (E4M3) {
           const int e = vmax[(n % FAC) * 4];
           if (t == p.t0) ev = e;
-          if (e > ev + V_RESCALE) {
-            alpha_o *= pow2(max(ev - e, -126));
+          if (e > ev + V_LAG) {
+            alpha_o = pow2(max(ev - e, -126));
             ev = e;
             grow = true;
           }
-          // this tile's V scale relative to the reference goes into the exponent
-          const int de = max(e - ev, -100);
-          ref -= (float)de;
+          const int de = max(e - ev, -100);  // goes into the exponent, and out of the sum again
+          shift = (float)de;
           back = pow2(-de);
+        }
+        // maximum first, then P, each a loop over 32 scores. One pass over all 64 with a second one
+        // when the maximum grew was slower: its code is fetched faster than the instruction cache
+        // gives it (e4m3, 32 x 14000 keys, 21 nodes: 760 us, these loops 552).
+        if (warp_on) {
+          float mt = -INFINITY;
+#pragma unroll 1
+          for (int c0 = 0; c0 < 64; c0 += 32) {
+            float x[32];
+            scores(c0, x);
+            float mx[2] = {x[0], x[1]};
+#pragma unroll
+            for (int c = 2; c < 32; ++c) mx[c & 1] = fmaxf(mx[c & 1], x[c]);
+            mt = fmaxf(mt, fmaxf(mx[0], mx[1]));
+          }
+          mt = fmaxf(mt, exchange(xmax + sb * 2 * BM, mt));
+          const float top = mt * rs - (E4M3 ? OFFSET8 : 0.f);
+          if (live && top > m + (E4M3 ? LAG8 : LAG)) {
+            const float f = sm100::exp2_approx(m - top);  // 0 on the first tile
+            alpha_o *= f;
+            l *= f;
+            m = top;
+            grow = true;
+          }
         }
         // rescale O rows once the previous PV completed (warp-wide, rare after the first tiles)
         if (__any_sync(0xffffffff, warp_on && grow && t > p.t0)) {
@@ -808,24 +831,39 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
           }
         }
         if (warp_on) {
-          float ps[2] = {0.f, 0.f};
+          const float ref = (m == -INFINITY ? 0.f : m) - shift;
+          float sum[2] = {0.f, 0.f};
+#pragma unroll 1
+          for (int c0 = 0; c0 < 64; c0 += 32) {
+            float x[32];
+            uint32_t pk[32];
+            scores(c0, x);
+            uint4 vw[4];
+            if constexpr (E4M3) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t hi[16], lo[16];
-            if constexpr (E4M3) scores(h * 32, x[0]);
+              for (int c = 0; c < 4; ++c) vw[c] = lds4(vf + (c0 + c * 8) * 2);
+            }
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
               float pr[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) pr[i] = sm100::exp2_approx(fmaf(x[h * (C::PP - 1)][c + i], rs, -ref));
-              ps[0] += pr[0] + pr[1];
-              ps[1] += pr[2] + pr[3];
+              for (int i = 0; i < 4; ++i) pr[i] = sm100::exp2_approx(fmaf(x[c + i], rs, -ref));
+              sum[0] += pr[0] + pr[1];
+              sum[1] += pr[2] + pr[3];
               if constexpr (E4M3) {
-                const float4 f = *reinterpret_cast<const float4*>(vf + h * 32 + c);
-                const __half2 h0 = __floats2half2_rn(pr[0] * f.x, pr[1] * f.y);
-                const __half2 h1 = __floats2half2_rn(pr[2] * f.z, pr[3] * f.w);
-                hi[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
-                hi[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+                const uint4 f = vw[c / 8];
+                const uint32_t f0 = c % 8 ? f.z : f.x, f1 = c % 8 ? f.w : f.y;
+                const __half2 h0 = __hmul2(__floats2half2_rn(pr[0], pr[1]), *reinterpret_cast<const __half2*>(&f0));
+                const __half2 h1 = __hmul2(__floats2half2_rn(pr[2], pr[3]), *reinterpret_cast<const __half2*>(&f1));
+                uint32_t w0 = *reinterpret_cast<const uint32_t*>(&h0), w1 = *reinterpret_cast<const uint32_t*>(&h1);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {  // the high byte of an f16 is an e5m2
+                  pk[y * 8 + c / 4] = __byte_perm(w0, w1, 0x7531);
+                  if (y < 3) {
+                    w0 = high_bytes_off(w0);
+                    w1 = high_bytes_off(w1);
+                  }
+                }
               } else {
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
@@ -833,54 +871,59 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
                   const uint32_t w = *reinterpret_cast<const uint32_t*>(&h2);
                   const __nv_bfloat162 l2 = __floats2bfloat162_rn(pr[i] - __uint_as_float(w << 16),
                                                                   pr[i + 1] - __uint_as_float(w & 0xffff0000u));
-                  hi[(c + i) / 2] = w;
-                  lo[(c + i) / 2] = *reinterpret_cast<const uint32_t*>(&l2);
+                  pk[(c + i) / 2] = w;
+                  pk[16 + (c + i) / 2] = *reinterpret_cast<const uint32_t*>(&l2);
                 }
               }
             }
-            sm100::tmem_st16_async(scol + h * 16, hi);  // over this thread's own scores
-            if constexpr (!E4M3) sm100::tmem_st16_async(scol + 32 + h * 16, lo);
+            sm100::tmem_st32_async(scol + c0, pk);  // over the scores just read
           }
-          l += (ps[0] + ps[1]) * back;
+          l += (sum[0] + sum[1]) * back;
           sm100::tmem_st_wait();
         }
         sm100::tc_fence_before();
         __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&p_full[sb]);
+        if (lane == 0) {
+          sm100::mbar_arrive(&p_full[sb]);
+          if constexpr (E4M3) sm100::mbar_arrive(&f_free[n % FAC]);
+        }
       }
-      // the gate, read while the last products run
+      // the gate, read 32 channels ahead: the first while the last products run
       const bool gated = a.gate && live && p.whole;
-      uint4 gw[DT / 16];
-      if (gated) {
-        const bf16* gt = a.gate + p.s * a.g_bs + tok * a.g_ts + hq * a.g_hs + half * (DT / 2);
+      uint4 gw[4];
+      auto read_gate = [&](int c) {
 #pragma unroll
-        for (int c = 0; c < DT / 16; ++c)
-          gw[c] = half * (DT / 2) + c * 8 < a.D ? *reinterpret_cast<const uint4*>(gt + c * 8) : make_uint4(0, 0, 0, 0);
-      }
+        for (int i = 0; i < 4; ++i)
+          if (gated && c + i * 8 < a.D)
+            gw[i] = *reinterpret_cast<const uint4*>(a.gate + p.s * a.g_bs + tok * a.g_ts + hq * a.g_hs + c + i * 8);
+      };
+      read_gate(half * (DT / 2));
       wait_all(o_last, pc & 1);
       sm100::tc_fence_after();
       if (warp_on) {
         l += exchange(xsum + (pc & 1) * 2 * BM, l);
         // O -> the output (a whole segment) or the workspace
-        const float vs = E4M3 ? pow2(ev + 8) : 1.f;
+        const float vs = E4M3 ? pow2(ev) : 1.f;
         const float inv = l > 0.f ? vs / l : (l == 0.f ? 0.f : l);
         // a CTA has one part that begins a segment (slot 1) and one that goes on with one (0) at most
         const int slot = p.t0 == 0;
         const int64_t at = ((int64_t)blockIdx.x * 2 + slot) * rows + row;
         bf16* o = a.out + (((int64_t)p.s * a.T + tok) * a.Hq + hq) * a.D;
-#pragma unroll
-        for (int c0 = 0; c0 < DT / 2; c0 += 32) {
-          const int c = half * (DT / 2) + c0;
+#pragma unroll 1
+        for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32) {
           float v[32];
           sm100::tmem_ld32(tmem + lane_off + c, v);
           if (!in) continue;
           if (p.whole) {
+            uint4 gc[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) gc[i] = gw[i];
+            if (c + 32 < (half + 1) * (DT / 2)) read_gate(c + 32);
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
               if (c + i < a.D) {
                 uint32_t w[4];
-                const uint4 g4 = gw[(c0 + i) / 8];
-                const uint32_t gg[4] = {g4.x, g4.y, g4.z, g4.w};
+                const uint32_t gg[4] = {gc[i / 8].x, gc[i / 8].y, gc[i / 8].z, gc[i / 8].w};
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                   float o0 = v[i + j] * inv, o1 = v[i + j + 1] * inv;
@@ -921,157 +964,114 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
       ++pc;
     }
   } else if constexpr (E4M3) {
-    // ---------------------------------------------------------- converters
-    // Per tile: the scales' factors (and, for the nodes' own tile, K as two matrices) in
-    // the place of S, V's f16 rows in the place of PV.
+    // ---------------------------------------------------------- scales, and the nodes' own rows
+    // Per tile: the scales' factors in the place of S. Of the nodes' tile also K (in the place of S)
+    // and V (of PV) as two 8-bit matrices of 64 rows each, one row per warp pass, four under way.
     const int cw = warp - 2 - SOFT_WARPS;
-    Ring kr, rr, vr;
+    Ring r;
     int n = 0;
     bool ok = true;
-    // 16-byte chunk of a node's row, and the exponent that brings the row into [2^at, 2^(at+1))
-    auto node_row = [&](const bf16* x, int at, uint4& w) -> int {
-      w = make_uint4(0, 0, 0, 0);
-      if (lane * 8 < a.D) w = *reinterpret_cast<const uint4*>(x + lane * 8);
-      return row_exponent(__reduce_max_sync(0xffffffff, finite_top(w)), at);
-    };
     auto wait_all = [&](uint64_t* bar, uint32_t parity) {
       if (lane == 0) ok = ok && wait(bar, parity, a.err);
       __syncwarp();
     };
     while (walk.next(a, p)) {
       product_order(p.t0, p.t1, [&](int t, bool pv) {
-        const int keys = p.keys(t);
+        const int keys = p.keys(t), fb = n % FAC;
         const bool own = t == p.nt;
-        const bf16* nv = a.v + p.s * a.v_bs + p.hk * a.v_hs;
-        if (!pv) {
-          const int fb = n % FAC;
-          if (own) {
-            const Ring k0 = kr;
-            for (int j = 0; j < KS; ++j) {
-              wait_all(&k_empty[kr.st], kr.ph ^ 1);
-              kr.step(NK);
-            }
-            uint8_t* hi_at = sK + k0.st * SLOT;
-            uint8_t* lo_at = DT == 256 ? sK + ((k0.st + 1) % NK) * SLOT : hi_at + MAX_NODES * 128;
-            for (int r = cw; r < MAX_NODES; r += CONV_WARPS) {
-              uint4 w = make_uint4(0, 0, 0, 0);
-              int e = EXP_MIN;
-              if (r < keys) e = node_row(a.k + p.s * a.k_bs + p.hk * a.k_hs + r * a.k_ts, 7, w);
-              uint2 hi, lo;
-              split_fp8(w, pow2(-e), hi, lo);
-              if (lane < DT / 8) {
-                const uint32_t at = tile_offset(MAX_NODES, r, lane >> 1) + (lane & 1) * 8;
-                *reinterpret_cast<uint2*>(hi_at + at) = hi;
-                *reinterpret_cast<uint2*>(lo_at + at) = lo;
-              }
-              if (lane == 0) kfac[fb * BN + r] = r < keys ? pow2(e) : 0.f;
-            }
-            sm100::fence_proxy_async_smem();
-            sm100::named_sync(5, CONV_WARPS * 32);
-            if (cw == 0) {
-              if (lane == 0) {
-                sm100::mbar_arrive(&k_full[k0.st]);
-                if (KS == 2) sm100::mbar_arrive(&k_full[(k0.st + 1) % NK]);
-              }
-              // V: the largest exponent, then every row's relative to it
-              int top = EXP_MIN, mine[2] = {EXP_MIN, EXP_MIN};
-              uint4 w;
-              for (int r = 0; r < keys; ++r) {
-                const int e = node_row(nv + r * a.v_ts, 8, w);
-                top = max(top, e);
-                if ((r & 31) == lane) mine[r >> 5] = e;
-              }
+        if (!own) {
+          for (int i = 0; i * VK < (pv ? keys : BN); ++i) r.step(NK);
+          if (pv) return;
+          if (cw == n % CONV_WARPS) {
+            if (n >= FAC) wait_all(&f_free[fb], (n / FAC - 1) & 1);
+            wait_all(&e_full[fb], (n / FAC) & 1);
+            const uint8_t* ex = sExp + fb * 2 * BN;
+            int e[4], top = EXP_MIN;
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                vfac[fb * BN + i * 32 + lane] = i * 32 + lane < keys ? pow2(max(mine[i & 1] - top, -126)) : 0.f;
-#pragma unroll
-              for (int i = 2; i < 4; ++i) kfac[fb * BN + i * 32 + lane] = 0.f;
-              __syncwarp();
-              if (lane == 0) {
-                vmax[fb * 4] = top;
-                sm100::mbar_arrive(&e_full[fb]);  // keeps its phase in step with the tiles
-                sm100::mbar_arrive(&f_full[fb]);
-              }
+            for (int i = 0; i < 4; ++i) {
+              const int x = lane + 32 * i;
+              kfac[fb * BN + x] = __float2bfloat16(x < keys ? pow2(min(max((int)ex[x] - EXP_BIAS, EXP_MIN), EXP_MAX)) : 0.f);
+              e[i] = min(max((int)ex[BN + x] - EXP_BIAS, EXP_MIN), EXP_MAX);
+              if (x < keys) top = max(top, e[i]);
             }
-          } else {
-            for (int j = 0; j < KS; ++j) kr.step(NK);
-            if (cw == n % CONV_WARPS) {
-              wait_all(&e_full[fb], (n / FAC) & 1);
-              const uint8_t* ex = sExp + fb * 2 * BN;
-              int e[4], top = EXP_MIN;
+            top = __reduce_max_sync(0xffffffff, top);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int r = lane + 32 * i;
-                kfac[fb * BN + r] = r < keys ? pow2(min(max((int)ex[r] - EXP_BIAS, EXP_MIN), EXP_MAX)) : 0.f;
-                e[i] = min(max((int)ex[BN + r] - EXP_BIAS, EXP_MIN), EXP_MAX);
-                if (r < keys) top = max(top, e[i]);
-              }
-              top = __reduce_max_sync(0xffffffff, top);
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                vfac[fb * BN + lane + 32 * i] = lane + 32 * i < keys ? pow2(max(e[i] - top, -126)) : 0.f;
-              if (lane == 0) vmax[fb * 4] = top;
-              __syncwarp();
-              if (lane == 0) sm100::mbar_arrive(&f_full[fb]);
-            }
+            for (int i = 0; i < 4; ++i)
+              vfac[fb * BN + lane + 32 * i] = __float2half(lane + 32 * i < keys ? pow2(max(e[i] - top, -126)) : 0.f);
+            if (lane == 0) vmax[fb * 4] = top;
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&f_full[fb]);
           }
           ++n;
-        } else if (own) {
-          for (int i = 0; i * VK < keys; ++i) {
-            wait_all(&v_empty[vr.st], vr.ph ^ 1);
-            uint8_t* tile = sV + vr.st * SLOT;
-            for (int r = cw; r < min(VK, (keys - i * VK + 15) & ~15); r += CONV_WARPS) {
-              uint4 w = make_uint4(0, 0, 0, 0);
-              if (i * VK + r < keys) {
-                const int e = node_row(nv + (i * VK + r) * a.v_ts, 8, w);
-                w = scale_to_f16(w, pow2(-8 - e));  // value * 2^-8 like the codes
-              }
-              if (lane < DT / 8) *reinterpret_cast<uint4*>(tile + tile_offset(VK, r, lane)) = w;
+          return;
+        }
+        if (pv && keys == 0) return;
+        const Ring r0 = r;
+        for (int j = 0; j < DA; ++j) {
+          wait_all(&empty[r.st], r.ph ^ 1);
+          r.step(NK);
+        }
+        if (!pv && n >= FAC) wait_all(&f_free[fb], (n / FAC - 1) & 1);
+        uint8_t* hi_at = sKV + r0.st * SLOT;
+        uint8_t* lo_at = DT == 256 ? sKV + (r0.st + 1) % NK * SLOT : hi_at + MAX_NODES * 128;
+        const bf16* ks = a.k + p.s * a.k_bs + p.hk * a.k_hs + lane * 8;
+        const bf16* vs = a.v + p.s * a.v_bs + p.hk * a.v_hs + lane * 8;
+#pragma unroll 1
+        for (int x0 = cw; x0 < MAX_NODES; x0 += 4 * CONV_WARPS) {
+          uint4 k4[4], v4[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int x = x0 + y * CONV_WARPS;
+            k4[y] = v4[y] = make_uint4(0, 0, 0, 0);
+            if (x < keys && lane * 8 < a.D) {
+              if (!pv) k4[y] = *reinterpret_cast<const uint4*>(ks + x * a.k_ts);
+              v4[y] = *reinterpret_cast<const uint4*>(vs + x * a.v_ts);
             }
-            sm100::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) sm100::mbar_arrive(&v_full[vr.st]);
-            vr.step(NV);
           }
-        } else {
-          const int r8 = lane >> 2, q4 = lane & 3;  // row of 8, 16 codes of 64
-          for (int i = 0; i * VK < keys; ++i) {
-            constexpr int PER = C::RK / VK;  // f16 slots that one slot of codes fills
-            if (i % PER == 0) wait_all(&r_full[rr.st], rr.ph);
-            wait_all(&v_empty[vr.st], vr.ph ^ 1);
-            const uint8_t* raw = sRaw + rr.st * SLOT + (i % PER) * VK * 64;
-            uint8_t* tile = sV + vr.st * SLOT;
-#pragma unroll 4
-            for (int x = cw; x < DA * (VK / 8); x += CONV_WARPS) {  // 8 rows x 64 channels at a time
-              const int j = x % DA, r = (x / DA) * 8 + r8;
-              uint4 w = *reinterpret_cast<const uint4*>(raw + j * (C::RK * 64) + r * 64 + q4 * 16);
-              if (i * VK + r >= keys) w = make_uint4(0, 0, 0, 0);
-              const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-              uint2 h[4];
 #pragma unroll
-              for (int y = 0; y < 4; ++y) h[y] = codes_to_f16(in[y]);
-              if ((nan_codes(w.x) | nan_codes(w.y)) | (nan_codes(w.z) | nan_codes(w.w))) {
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                  const uint32_t z = nan_codes(in[y]) >> 7;  // 1 in the byte of each NaN
-                  h[y].x |= ((z & 1) | ((z & 0x100) << 8)) * 0x7fffu;
-                  h[y].y |= (((z >> 16) & 1) | ((z >> 16 & 0x100) << 8)) * 0x7fffu;
-                }
+          for (int y = 0; y < 4; ++y) {
+            const int x = x0 + y * CONV_WARPS;
+            int e;
+            if (!pv) {  // exponents that bring the rows into [2^7, 2^8)
+              e = x < keys ? row_exponent(__reduce_max_sync(0xffffffff, finite_top(k4[y])), 7) : EXP_MIN;
+              const int ve = row_exponent(__reduce_max_sync(0xffffffff, finite_top(v4[y])), 7);
+              if (lane == 0) {
+                kfac[fb * BN + x] = __float2bfloat16(x < keys ? pow2(e) : 0.f);
+                vexp[x] = x < keys ? ve : EXP_MIN;
               }
-              const int c = j * 8 + q4 * 2;
-              *reinterpret_cast<uint4*>(tile + tile_offset(VK, r, c)) = make_uint4(h[0].x, h[0].y, h[1].x, h[1].y);
-              *reinterpret_cast<uint4*>(tile + tile_offset(VK, r, c + 1)) = make_uint4(h[2].x, h[2].y, h[3].x, h[3].y);
+            } else {
+              e = vexp[x];
             }
-            sm100::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              sm100::mbar_arrive(&v_full[vr.st]);
-              if (i % PER == PER - 1 || (i + 1) * VK >= keys) sm100::mbar_arrive(&r_empty[rr.st]);
+            uint2 hi, lo;
+            split_fp8(pv ? v4[y] : k4[y], pow2(-e), hi, lo);
+            if (lane < DT / 8) {
+              const uint32_t at = tile_offset(MAX_NODES, x, lane >> 1) + (lane & 1) * 8;
+              *reinterpret_cast<uint2*>(hi_at + at) = hi;
+              *reinterpret_cast<uint2*>(lo_at + at) = lo;
             }
-            if (i % PER == PER - 1 || (i + 1) * VK >= keys) rr.step(NR);
-            vr.step(NV);
           }
         }
+        sm100::fence_proxy_async_smem();
+        sm100::named_sync(5, CONV_WARPS * 32);
+        if (cw == 0) {
+          if (lane < DA) sm100::mbar_arrive(&full[(r0.st + lane) % NK]);
+          if (!pv) {  // V's factors relative to the largest
+            const int e0 = vexp[lane], e1 = vexp[lane + 32];
+            const int top = __reduce_max_sync(0xffffffff, max(lane < keys ? e0 : EXP_MIN, lane + 32 < keys ? e1 : EXP_MIN));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              vfac[fb * BN + i * 32 + lane] = __float2half(i * 32 + lane < keys ? pow2(max((i ? e1 : e0) - top, -126)) : 0.f);
+              if (i >= 2) kfac[fb * BN + i * 32 + lane] = __float2bfloat16(0.f);
+            }
+            if (lane == 0) vmax[fb * 4] = top;
+            __syncwarp();
+            if (lane == 0) {
+              sm100::mbar_arrive(&e_full[fb]);  // keeps its phase in step with the tiles
+              sm100::mbar_arrive(&f_full[fb]);
+            }
+          }
+        }
+        if (!pv) ++n;
       });
     }
   }
@@ -1172,8 +1172,7 @@ CUtensorMap pool_map(const void* base, const CacheView& c, int cols, int rows) {
   cuuint64_t dims[2] = {(cuuint64_t)c.d, (cuuint64_t)n}, strides[1] = {(cuuint64_t)c.d};
   cuuint32_t box[2] = {(cuuint32_t)cols, (cuuint32_t)rows}, estr[2] = {1, 1};
   CUresult r = encode_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   NS_CHECK(r == CUDA_SUCCESS, "tree_attention: cuTensorMapEncodeTiled failed");
   return map;
@@ -1188,8 +1187,7 @@ void launch(const Args& a, int grid, const CacheView& c, const at::Tensor& q, co
     NS_CUDA(cudaFuncSetAttribute(tree_attn_kernel<DT, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
   });
   const CUtensorMap tq = node_map(q, a.GT, a.TPM), tk = node_map(k, 1, a.T), tv = node_map(v, 1, std::min(a.T, C::VK)),
-                    tkp = pool_map(c.k, c, E4M3 ? 128 : 64, std::min(c.page, BN)),
-                    tvp = pool_map(c.v, c, 64, std::min(c.page, E4M3 ? C::RK : C::VK));
+                    tkp = pool_map(c.k, c, C::AC, std::min(c.page, BN)), tvp = pool_map(c.v, c, C::AC, std::min(c.page, C::VK));
   tree_attn_kernel<DT, E4M3><<<grid, C::THREADS, C::SMEM, stream()>>>(tq, tk, tv, tkp, tvp, a);
   NS_CUDA(cudaGetLastError());
 }
