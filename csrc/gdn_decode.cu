@@ -25,6 +25,11 @@
 // (mma.sync and not tcgen05: the fp32 state has to be split in registers anyway, and at the
 // sizes of a decoding step the loads of S dominate.) The unit triangular system in u is
 // solved by blocks of 16 nodes in fp32.
+//
+// Measured (48 heads of 128): one token of 64 sequences 75 us and short paths 76 us (5.4 TB/s,
+// 84 % of the copy rate), the states' bytes. Trees: 16 sequences x 16 nodes 42 us, 32 x 61 nodes
+// 244 us (0.9 TB/s): a CTA's phases wait for one another (loads, S K, M, solve, A u) with 12
+// warps an SM to hide it, 3 CTAs by registers.
 #include "decode.h"
 #include "sm100.cuh"
 

@@ -1016,8 +1016,9 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
         uint8_t* lo_at = DT == 256 ? sKV + (r0.st + 1) % NK * SLOT : hi_at + MAX_NODES * 128;
         const bf16* ks = a.k + p.s * a.k_bs + p.hk * a.k_hs + lane * 8;
         const bf16* vs = a.v + p.s * a.v_bs + p.hk * a.v_hs + lane * 8;
+        const int rows = (keys + 31) & ~31;  // up to the edge of the last product with P
 #pragma unroll 1
-        for (int x0 = cw; x0 < MAX_NODES; x0 += 4 * CONV_WARPS) {
+        for (int x0 = cw; x0 < rows; x0 += 4 * CONV_WARPS) {
           uint4 k4[4], v4[4];
 #pragma unroll
           for (int y = 0; y < 4; ++y) {

@@ -11,8 +11,9 @@ CUDA tensors run the sm_100a kernels of ``nanospec_b200._C`` on the current stre
 activations, fp32 decays and states); CPU tensors run the statements in
 ``ops.reference``. Bad shapes, types and layouts raise ``ValueError``. Bad *values* of
 index tensors (slots, page tables, lengths, parents, counts, paths) cannot be seen without
-waiting for the GPU: there the kernels skip the access and set the device error
-word (code 4, see ``utils.health``); on the CPU they raise ``IndexError``.
+waiting for the GPU: there the kernels skip the access (a page that does not exist is
+replaced by page 0 in ``tree_attention``) and set the device error word (code 4, see
+``utils.health``); on the CPU they raise ``IndexError``.
 
 Index tensors are int32 (``slots`` int64). Nodes at or beyond ``counts`` are padding: their
 inputs are not used, their outputs are zeros (lse -inf).
@@ -143,6 +144,8 @@ def tree_attention(q, k, v, cache, table, lens, parents, counts=None, gate=None,
     Node t sees positions [0, lens) and itself and its ancestors. ``gate`` [b, T, Hq, D],
     when given, multiplies the output by sigmoid(gate); ``scale`` defaults to D^-1/2.
     Strided views are taken as they are when D is contiguous and rows are 16-byte aligned.
+    Live nodes' k and v must be finite: a product with a masked one's zero probability is
+    still formed. (Whatever lies in pages beyond ``lens`` or in padding nodes is not used.)
 
     Returns (out [b, T, Hq, D], lse [b, Hq, T] fp32, natural log, before the gate).
     """
