@@ -16,8 +16,8 @@
 //
 // Work is split over the long axis without knowing the lengths on the host: the tiles of
 // all segments (sequence, key head, row tile) are numbered through, and CTA i of N (one per
-// SM) takes units [U i / N, U (i+1) / N) (every segment counts two more for its beginning and
-// end), so ragged batches and single long sequences load
+// SM) takes units [U i / N, U (i+1) / N) (every segment counts a few more for its beginning
+// and end), so ragged batches and single long sequences load
 // every SM alike. A segment that one CTA holds whole is finished there; parts of a segment
 // leave unnormalised O with its reference maximum and sum in a workspace (two parts per CTA
 // at most), and tree_join_kernel adds them up in the order of the CTAs.
@@ -62,7 +62,6 @@ constexpr float LAG8 = 6.f;           // e4m3: by this, the reference V exponent
 constexpr int V_LAG = 1;              // probabilities are at most 2^(OFFSET8 + 6 + 1) = 2^15, the top of
 constexpr float OFFSET8 = 8.f;        // e5m2, whose smallest step, 2^-16, is 2^-24 of the largest then
 constexpr int SLOT = 16384;           // bytes of one ring slot
-constexpr int SEG_UNITS = 2;          // what beginning and ending a segment costs, in tiles
 constexpr int SOFT_WARPS = 8, CONV_WARPS = 2;
 
 struct Args {
@@ -72,6 +71,7 @@ struct Args {
   const int *table, *lens, *parents, *counts;
   int64_t p_bs, pages, max_pages;
   int b, T, Hq, Hk, D, page, page_log2;
+  int seg;                // what beginning and ending a segment costs, in tiles
   int G, GT, HB, TPM, M;  // heads of a group, per row tile, head blocks; tokens per row tile, token blocks
   float scale_log2;
   bf16* out;    // [b, T, Hq, D]
@@ -121,10 +121,10 @@ __device__ __forceinline__ Seq sequence(const Args& a, int s, bool flag) {
 }
 
 // Units of work: a row tile whose first token is live has the prefix's tiles and the nodes',
-// others one tile of zeros; every segment starts with SEG_UNITS that stand for its beginning
+// others one tile of zeros; every segment starts with `seg` units that stand for its beginning
 // and end (q, first loads, output).
 __device__ __forceinline__ int64_t group_units(const Args& a, Seq q, int live) {
-  return (int64_t)live * ((q.len + BN - 1) / BN + 1 + SEG_UNITS) + (int64_t)(a.M - live) * (1 + SEG_UNITS);
+  return (int64_t)live * ((q.len + BN - 1) / BN + 1 + a.seg) + (int64_t)(a.M - live) * (1 + a.seg);
 }
 __device__ __forceinline__ int64_t seq_units(const Args& a, Seq q) {
   return (int64_t)a.Hk * a.HB * group_units(a, q, (q.cnt + a.TPM - 1) / a.TPM);
@@ -161,11 +161,11 @@ struct Walk {
       p.hk = seg / (a.M * a.HB);
       p.own = p.m * a.TPM < q.cnt ? q.cnt : 0;
       p.nt = p.own > 0 ? (q.len + BN - 1) / BN : 0;
-      const int units = p.nt + 1 + SEG_UNITS;
+      const int units = p.nt + 1 + a.seg;
       p.last = unit - off + units - 1;
       const int to = (int)min((int64_t)units, off + (end - unit));
-      p.t0 = max(off - SEG_UNITS, 0);
-      p.t1 = max(to - SEG_UNITS, 0);
+      p.t0 = max(off - a.seg, 0);
+      p.t1 = max(to - a.seg, 0);
       p.whole = p.t0 == 0 && p.t1 == p.nt + 1;
       unit += to - off;
       off = to;
@@ -215,7 +215,7 @@ __device__ __forceinline__ Walk plan(const Args& a, int lane, int64_t& U, int& N
       w.q.len = __shfl_sync(0xffffffff, q.len, l);
       w.q.cnt = __shfl_sync(0xffffffff, q.cnt, l);
       const int live = (w.q.cnt + a.TPM - 1) / a.TPM;
-      const int64_t units = (w.q.len + BN - 1) / BN + 1 + SEG_UNITS;
+      const int64_t units = (w.q.len + BN - 1) / BN + 1 + a.seg;
       const int64_t group = group_units(a, w.q, live);  // one (key head, head block)
       w.seg = (int)(rem / group) * a.M;
       rem %= group;
@@ -224,8 +224,8 @@ __device__ __forceinline__ Walk plan(const Args& a, int lane, int64_t& U, int& N
         w.off = (int)(rem % units);
       } else {
         rem -= live * units;
-        w.seg += live + (int)(rem / (1 + SEG_UNITS));
-        w.off = (int)(rem % (1 + SEG_UNITS));
+        w.seg += live + (int)(rem / (1 + a.seg));
+        w.off = (int)(rem % (1 + a.seg));
       }
       break;
     }
@@ -1256,6 +1256,9 @@ std::vector<at::Tensor> tree_attention(at::Tensor q, at::Tensor k, at::Tensor v,
   a.pages = c.pages, a.max_pages = table.size(1);
   a.b = (int)b, a.T = (int)T, a.Hq = (int)Hq, a.Hk = c.heads, a.D = (int)D, a.page = c.page;
   a.page_log2 = c.page == 16 ? 4 : c.page == 32 ? 5 : c.page == 64 ? 6 : 7;
+  // measured at 2 and 4 (us): e4m3, one node of 64 ragged sequences, 479 and 448, bf16 short
+  // trees 65 and 72; an e4m3 segment also splits the nodes' rows
+  a.seg = c.e4m3 ? 4 : 2;
   a.G = (int)Hq / c.heads;
   a.HB = (a.G + tattn::BM - 1) / tattn::BM;
   a.GT = (a.G + a.HB - 1) / a.HB;
