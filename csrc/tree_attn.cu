@@ -252,7 +252,7 @@ struct Cfg {
   static constexpr int PP = E4M3 ? 4 : 2;          // matrices whose sum is P
   static constexpr int Q_BYTES = BM * DT * 2;      // bf16, or the two 8-bit matrices
   static constexpr int NK = DT == 256 ? 9 : 11;    // ring slots, K and V in the order of the products
-  static constexpr int XCH = 2 * 2 * 2 * BM * 4;   // maxima and sums exchanged by a row's two threads
+  static constexpr int XCH = 3 * 2 * 2 * BM * 4;   // maxima, sums and q's maxima exchanged by a row's threads
   // e4m3 scales of FAC tiles: exponent bytes, K and V factors, largest V exponent
   static constexpr int FAC = 4;
   static constexpr int FACS = E4M3 ? FAC * (2 * BN + 2 * BN * 2 + 16) + MAX_NODES * 4 : 0;
@@ -341,7 +341,8 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
   uint8_t* sExp = reinterpret_cast<uint8_t*>(vexp + (E4M3 ? MAX_NODES : 0));  // [FAC][2][BN] exponent bytes
   float* xmax = reinterpret_cast<float*>(sExp + (E4M3 ? FAC * 2 * BN : 0));   // [2][2][BM]
   float* xsum = xmax + 2 * 2 * BM;                                            // [2][2][BM]
-  int* page_rows = reinterpret_cast<int*>(xsum + 2 * 2 * BM);                 // [4][8] of the producer
+  float* xq = xsum + 2 * 2 * BM;                                              // [2][2][BM]
+  int* page_rows = reinterpret_cast<int*>(xq + 2 * 2 * BM);                 // [4][8] of the producer
   uint64_t* bars = reinterpret_cast<uint64_t*>(page_rows + 32);
   uint64_t* full = bars;             // [NK]
   uint64_t* empty = full + NK;       // [NK]
@@ -708,7 +709,7 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
 #pragma unroll
             for (int c = 0; c < 8; ++c) top = max(top, finite_top(w[c]));
           }
-          top = max(top, __float_as_uint(exchange(xsum + (pc & 1 ^ 1) * 2 * BM, __uint_as_float(top))));
+          top = max(top, __float_as_uint(exchange(xq + (pc & 1) * 2 * BM, __uint_as_float(top))));
           const int e = row_exponent(top, 7);
           rs *= pow2(e);
           const float sc = pow2(-e);
