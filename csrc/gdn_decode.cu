@@ -341,7 +341,8 @@ __global__ void __launch_bounds__(Nodes<D, NT>::THREADS, 3) gdn_nodes_kernel(Arg
       }
     }
     __syncthreads();  // decays are complete
-    if (!TREE && tid < TP) cf[tid] = ik[tid] * mt[tid * MS + TP - 1];
+    if constexpr (!TREE)  // (a CTA of narrow heads has fewer threads than nodes)
+      for (int t = tid; t < TP; t += C::THREADS) cf[t] = ik[t] * mt[t * MS + TP - 1];
     // right-hand sides beta (v - w S^T k^)
 #pragma unroll
     for (int j = 0; j < NT; ++j)
