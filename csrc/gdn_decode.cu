@@ -910,7 +910,7 @@ void gdn_accept(at::Tensor k, at::Tensor g, at::Tensor u, at::Tensor path, at::T
   NS_VALUE(d.b < 65536 && d.nv < 65536, "gated delta rule: too many sequences or heads");
   bind_state(d, state, rows, &out_state);
   if (d.b * d.nv == 0) return;
-  d.keep = {aligned_rows(k), g.stride(2) == 1 ? g : g.contiguous(), u.contiguous()};
+  d.keep = {aligned_rows(k), g.stride(2) == 1 ? g : g.contiguous(), aligned_dense(u)};
   d.a.k = bf_ptr(d.keep[0]);
   d.a.k_bs = d.keep[0].stride(0), d.a.k_ts = d.keep[0].stride(1), d.a.k_hs = d.keep[0].stride(2);
   d.a.g = d.keep[1].data_ptr<float>();

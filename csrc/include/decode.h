@@ -73,13 +73,21 @@ inline const int* check_parents(const at::Tensor& p, int64_t b, int64_t t, const
   return p.data_ptr<int>();
 }
 
+// Whether 16-byte accesses may start at t's first element.
+inline bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+// t, dense and 16-byte aligned: anything else is copied (`contiguous` alone keeps a dense view
+// that begins at an odd offset of its storage).
+inline at::Tensor aligned_dense(const at::Tensor& t) {
+  return t.is_contiguous() && aligned16(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 // A bf16 operand [.., heads, D] on `dev` as the kernels read it: D contiguous, every row
 // 16-byte aligned; anything else is copied.
 inline at::Tensor aligned_rows(const at::Tensor& t) {
-  bool ok = t.size(-1) <= 1 || t.stride(-1) == 1;
+  bool ok = (t.size(-1) <= 1 || t.stride(-1) == 1) && aligned16(t);
   for (int i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
-  ok = ok && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  return ok ? t : t.contiguous();
+  return ok ? t : aligned_dense(t);
 }
 
 }  // namespace ns

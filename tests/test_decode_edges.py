@@ -6,7 +6,7 @@ import torch
 
 from nanospec_b200.ops import decode_ops as dops
 
-from test_decode_ops import BF, Delta, _device_error, devices, near  # noqa: F401
+from test_decode_ops import BF, Delta, Problem, _device_error, devices, near  # noqa: F401
 
 NARROW = [(2, 33, 1, 2, 16, None), (1, 64, 2, 1, 16, None), (2, 70, 2, 2, 16, [70, 41]), (2, 131, 1, 1, 16, [97, 131]),
           (1, 70, 1, 1, 32, None), (1, 70, 1, 1, 64, None)]
@@ -23,3 +23,48 @@ def test_delta_advance_narrow_heads(dev, case):
     out, _ = dops.gated_delta_advance(*s.to("q", "k", "v", "g", "beta"), state, gr, counts=s.c())
     near(out, w_out, BF)
     near(state, torch.stack([states[i][max(states[i])] for i in range(b)]))
+
+
+def shifted(x, by):
+    """x, dense, at ``by`` elements into its storage."""
+    return x.new_empty(x.numel() + by)[by:].view(x.shape).copy_(x)
+
+
+@devices
+@pytest.mark.parametrize("by", [1, 4])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_dense_operands_at_odd_addresses(dev, by, e4m3):
+    """Dense views that begin off a 16-byte boundary give what aligned ones give."""
+    p = Problem(dev, [90, 33], 5, 8, 2, 64, 16, e4m3)
+    p.dev = [x.contiguous() for x in p.dev]
+    want = p.run()
+    p.dev = [shifted(x, by) for x in p.dev]
+    assert all(x.is_contiguous() and (dev == "cpu" or x.data_ptr() % 16) for x in p.dev)
+    assert all(torch.equal(a, b) for a, b in zip(p.run(), want))
+    k, v = (torch.randn(7, 2, 64, device=dev).bfloat16() for _ in range(2))
+    slots = torch.arange(7, device=dev) + p.table[1, 0] * 16
+    got = []
+    for a, b in ((k, v), (shifted(k, by), shifted(v, by))):
+        dops.cache_write(p.cache, a, b, slots)
+        got += [dops.cache_read(p.cache, p.table, p.lens, 7)]
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@devices
+@pytest.mark.parametrize("by", [1, 2])
+@pytest.mark.parametrize("t,d", [(1, 128), (20, 128), (40, 32)])
+def test_dense_delta_operands_at_odd_addresses(dev, by, t, d):
+    s = Delta(dev, 2, t, 1, 2, d)
+    q, k, v, g, beta, state, parents = s.to("q", "k", "v", "g", "beta", "state", "parents")
+    odd = [shifted(x, by) for x in (q, k, v, g, beta)]
+    want, got = state.clone(), state.clone()
+    a, b = dops.gated_delta_advance(q, k, v, g, beta, want, 2)[0], dops.gated_delta_advance(*odd, got, 2)[0]
+    assert torch.equal(a, b) and torch.equal(want, got)
+    a, b = (dops.gated_delta_verify(*x, state, parents, 2) for x in ((q, k, v, g, beta), odd))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    path = torch.arange(t, dtype=torch.int32, device=dev).expand(2, -1).contiguous()
+    for m in {1, t}:
+        want, got = torch.empty_like(state), torch.empty_like(state)
+        dops.gated_delta_accept(k, g, a[1], path[:, :m].contiguous(), state, 2, out_state=want)
+        dops.gated_delta_accept(odd[1], odd[3], shifted(a[1], by), path[:, :m].contiguous(), state, 2, out_state=got)
+        assert torch.equal(want, got)
