@@ -789,6 +789,16 @@ struct Delta {
 
 const bf16* bf_ptr(const at::Tensor& t) { return reinterpret_cast<const bf16*>(t.data_ptr()); }
 
+// No row of x (`row` fp32 each) shares memory with a row of y: their extents are apart, or rows of
+// one stride interleave.
+bool rows_apart(const at::Tensor& x, const at::Tensor& y, int64_t row) {
+  const int64_t n = x.size(0), sx = x.stride(0), sy = y.stride(0), off = y.data_ptr<float>() - x.data_ptr<float>();
+  if (n == 0 || off >= (n - 1) * sx + row || -off >= (n - 1) * sy + row) return true;
+  if (n == 1 || sx != sy || sx < 2 * row) return false;
+  const int64_t in = (off % sx + sx) % sx;
+  return in >= row && in + row <= sx;
+}
+
 void bind_state(Delta& d, const at::Tensor& state, const OptTensor& rows, const at::Tensor* out) {
   auto ok = [&](const at::Tensor& s) {
     return s.dim() == 4 && s.size(1) == d.nv && s.size(2) == d.D && s.size(3) == d.D && s.scalar_type() == at::kFloat &&
@@ -803,6 +813,11 @@ void bind_state(Delta& d, const at::Tensor& state, const OptTensor& rows, const 
   d.a.rows = check_index(rows, d.b, d.dev, "rows");
   if (out) {
     NS_VALUE(ok(*out) && out->size(0) == state.size(0), "gated delta rule: out_state must be like state");
+    // one CTA's rows must not be another's: out's own, and those of state unless it is state itself
+    const int64_t row = d.nv * d.D * d.D, n = state.size(0);
+    NS_VALUE(n <= 1 || out->stride(0) >= row, "gated delta rule: rows of out_state overlap");
+    const bool same = out->data_ptr() == state.data_ptr() && (n <= 1 || out->stride(0) == state.stride(0));
+    NS_VALUE(same || rows_apart(state, *out, row), "gated delta rule: out_state must be state or lie apart from it");
     d.a.out_state = out->data_ptr<float>();
     d.a.o_rs = out->stride(0);
   }

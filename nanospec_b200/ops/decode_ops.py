@@ -172,9 +172,10 @@ def gated_delta_advance(q, k, v, g, beta, state, groups=1, counts=None, rows=Non
     Like ``verifier_ops.gated_delta_rule`` (q, k [b, T, nk, D] raw, v [b, T, nv, D], g fp32
     and beta [b, T, nv], value head h using key head h // groups), but in fp32 throughout,
     starting from ``state`` fp32 [n, nv, D, D] (key channel, value channel). Sequence i
-    uses row ``rows[i]`` (None: i; -1: an idle sequence, zero outputs) and its first
-    ``counts[i]`` tokens. The new states go to the same rows of ``out_state`` (None: to
-    ``state``, in place). Returns (out [b, T, nv, D], out_state).
+    uses row ``rows[i]`` (None: i; -1: an idle sequence, zero outputs; rows must not repeat)
+    and its first ``counts[i]`` tokens. The new states go to the same rows of ``out_state``
+    (None: to ``state``, in place; otherwise memory apart from it). Returns
+    (out [b, T, nv, D], out_state).
     """
     out_state = state if out_state is None else out_state
     if q.is_cuda:
@@ -210,8 +211,8 @@ def gated_delta_verify(q, k, v, g, beta, state, parents, groups=1, counts=None, 
 def gated_delta_accept(k, g, u, path, state, groups=1, rows=None, out_state=None):
     """Move ``state`` on along the accepted nodes ``path`` [b, m <= 64] of a verified tree
     (root first, -1 entries skipped): S <- e^{g_a} S + k_a u_a^T. k and g as given to
-    ``gated_delta_verify``, u as it returned it. In place unless ``out_state`` is given;
-    returns the new states."""
+    ``gated_delta_verify``, u as it returned it. In place unless ``out_state`` (memory apart
+    from ``state``) is given; ``rows`` must not repeat. Returns the new states."""
     out_state = state if out_state is None else out_state
     if k.is_cuda:
         _c().gdn_accept(k, g, u, path, state, int(groups), rows, out_state)
@@ -279,6 +280,13 @@ def _check_delta(q, k, v, g, beta, state, groups):
 def _check_out_state(state, out_state):
     _need(out_state.shape == state.shape and out_state.dtype == state.dtype,
           "gated delta rule: out_state must be like state")
+    n, row, sx, sy = state.shape[0], state.shape[1:].numel(), state.stride(0), out_state.stride(0)
+    _need(n <= 1 or sy >= row, "gated delta rule: rows of out_state overlap")
+    off = (out_state.data_ptr() - state.data_ptr()) // 4
+    same = off == 0 and (n <= 1 or sx == sy)
+    apart = n == 0 or off >= (n - 1) * sx + row or -off >= (n - 1) * sy + row  # or rows interleave
+    apart = apart or (n > 1 and sx == sy >= 2 * row and row <= off % sx <= sx - row)
+    _need(same or apart, "gated delta rule: out_state must be state or lie apart from it")
 
 
 def _check_rows(rows, b, state):

@@ -6,7 +6,7 @@ import torch
 
 from nanospec_b200.ops import decode_ops as dops
 
-from test_decode_ops import BF, Delta, Problem, _device_error, devices, near  # noqa: F401
+from test_decode_ops import BF, Delta, Problem, _device_error, devices, i32, near  # noqa: F401
 
 NARROW = [(2, 33, 1, 2, 16, None), (1, 64, 2, 1, 16, None), (2, 70, 2, 2, 16, [70, 41]), (2, 131, 1, 1, 16, [97, 131]),
           (1, 70, 1, 1, 32, None), (1, 70, 1, 1, 64, None)]
@@ -68,3 +68,26 @@ def test_dense_delta_operands_at_odd_addresses(dev, by, t, d):
         dops.gated_delta_accept(k, g, a[1], path[:, :m].contiguous(), state, 2, out_state=want)
         dops.gated_delta_accept(odd[1], odd[3], shifted(a[1], by), path[:, :m].contiguous(), state, 2, out_state=got)
         assert torch.equal(want, got)
+
+
+@devices
+def test_out_states_that_overlap(dev):
+    """States move on in place or to memory of their own: a row being read is nobody's to write."""
+    s = Delta(dev, 3, 2, 1, 2, 16)
+    q, k, v, g, beta, state = s.to("q", "k", "v", "g", "beta", "state")
+    pool = torch.zeros(8, 2, 2, 16, 16, device=dev)
+    flat = pool[:, 0].contiguous()
+    u, path = torch.zeros(3, 2, 2, 16, device=dev), i32([[0, 1]] * 3, dev)
+    want = state.clone()
+    out = dops.gated_delta_advance(q, k, v, g, beta, want, 2)[0]
+    for a, b in ((flat[:3], flat[3:6]), (flat[5:], flat[2:5]), (pool[:3, 0], pool[:3, 1]), (pool[:3, 1], pool[:3, 0]),
+                 (pool[2:5, 1], pool[3:6, 0]), (flat[:3], flat[:3]), (pool[1:4, 1], pool[1:4, 1])):
+        a.copy_(state)
+        got, ret = dops.gated_delta_advance(q, k, v, g, beta, a, 2, out_state=b)
+        assert ret is b and torch.equal(got, out) and torch.equal(b, want)
+    for a, b in ((flat[:3], flat[1:4]), (flat[2:5], flat[:3]), (flat[:3], flat[:6:2]), (state, flat[:1].expand(3, -1, -1, -1)),
+                 (pool[:3, 0], flat.as_strided((3, 2, 16, 16), (256, 256, 16, 1)))):
+        with pytest.raises(ValueError):
+            dops.gated_delta_advance(q, k, v, g, beta, a, 2, out_state=b)
+        with pytest.raises(ValueError):
+            dops.gated_delta_accept(k, g, u, path, a, 2, out_state=b)
