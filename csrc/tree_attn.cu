@@ -19,7 +19,7 @@
 // SM) takes units [U i / N, U (i+1) / N) (every segment counts a few more for its beginning
 // and end), so ragged batches and single long sequences load
 // every SM alike. A segment that one CTA holds whole is finished there; parts of a segment
-// leave unnormalised O with its reference maximum and sum in a workspace (two parts per CTA
+// leave their output with its reference maximum and sum in a workspace (two parts per CTA
 // at most), and tree_join_kernel adds them up in the order of the CTAs.
 //
 // bf16 pages: P must be bf16 like V, whose 8 bits would cost as much as the output's own
@@ -31,8 +31,11 @@
 // exactly (elements below 2^-14 of the row's largest are held to 2^-22 of it). V's codes are
 // multiplied in 8 bits too: P as f16 (11 bits) is the sum of four e5m2 matrices, each the high
 // bytes of what the ones before left. The rows' scales stay outside the products: K's
-// multiplies the score, V's the probability, relative to the largest V scale seen so far
-// (when that grows by more than a factor of 2, O is rescaled like for a growing maximum). The nodes' own
+// multiplies the score, V's, 2^e_j, the probability: P_j = 2^(s_j + e_j - r) with r a running
+// maximum of s_j + e_j (log2) over the keys that the row sees, apart from that of s_j which
+// the sum is relative to. So a V row of any scale counts by what it adds to the output: terms below
+// 2^-28 of the row's largest 2^(s_j + e_j) are dropped (2^-28 of it at most per key, half a
+// rounding of the output at 2^18 such keys), the others keep 11 bits. The nodes' own
 // K and V are split like q. So no operand is converted on its way to the tensor cores.
 //
 // Measured (32 sequences of 14000 keys, 4 key heads of 256, pages of 64): bf16 390 us at one
@@ -57,10 +60,10 @@ namespace tattn {
 
 constexpr int EXP_BIAS = 127, EXP_MIN = -117, EXP_MAX = 118;
 constexpr int BM = 128, BN = 128;
-constexpr float LAG = 8.f;            // the reference maximum may lag by this much (log2); bf16
-constexpr float LAG8 = 6.f;           // e4m3: by this, the reference V exponent by V_LAG, and
-constexpr int V_LAG = 1;              // probabilities are at most 2^(OFFSET8 + 6 + 1) = 2^15, the top of
-constexpr float OFFSET8 = 8.f;        // e5m2, whose smallest step, 2^-16, is 2^-24 of the largest then
+constexpr float LAG = 8.f;      // the reference maximum of the scores may lag by this much (log2)
+constexpr float LAG8 = 3.f;     // e4m3: that of score and V scale together by this, so P is at most
+constexpr float OFFSET8 = 12.f; // 2^(OFFSET8 + LAG8) = 2^15, the top of e5m2, whose smallest step, 2^-16, is 2^-28
+                                // of the largest P when the reference has just been set
 constexpr int SLOT = 16384;           // bytes of one ring slot
 constexpr int SOFT_WARPS = 8, CONV_WARPS = 2;
 
@@ -76,7 +79,7 @@ struct Args {
   float scale_log2;
   bf16* out;    // [b, T, Hq, D]
   float* lse;   // [b, Hq, T]
-  float* part;  // [N][2][GT * TPM][D] unnormalised O
+  float* part;  // [N][2][GT * TPM][D] the parts' outputs
   float2* ml;   // [N][2][GT * TPM] reference maximum (log2) and sum
   int2* info;   // [segments] first CTA, last CTA
   int* err;
@@ -252,10 +255,11 @@ struct Cfg {
   static constexpr int PP = E4M3 ? 4 : 2;          // matrices whose sum is P
   static constexpr int Q_BYTES = BM * DT * 2;      // bf16, or the two 8-bit matrices
   static constexpr int NK = DT == 256 ? 9 : 11;    // ring slots, K and V in the order of the products
-  static constexpr int XCH = 3 * 2 * 2 * BM * 4;   // maxima, sums and q's maxima exchanged by a row's threads
-  // e4m3 scales of FAC tiles: exponent bytes, K and V factors, largest V exponent
+  // maxima, sums, q's maxima and those with V's scale exchanged by a row's threads
+  static constexpr int XCH = 4 * 2 * 2 * BM * 4;
+  // e4m3 scales of FAC tiles: exponent bytes, K's factors and V's exponents
   static constexpr int FAC = 4;
-  static constexpr int FACS = E4M3 ? FAC * (2 * BN + 2 * BN * 2 + 16) + MAX_NODES * 4 : 0;
+  static constexpr int FACS = E4M3 ? FAC * (2 * BN + 2 * BN * 2) + MAX_NODES * 4 : 0;
   static constexpr int SMEM = Q_BYTES + NK * SLOT + FACS + XCH + 128 + 512 + 1024;
   static constexpr int S_COL = DT;
   static constexpr int TMEM_COLS = 512;            // DT + 2 BN, a power of two
@@ -335,14 +339,14 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
   uint8_t* sQ = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sKV = sQ + C::Q_BYTES;                                        // [NK]
   bf16* kfac = reinterpret_cast<bf16*>(sKV + NK * SLOT);                 // [FAC][BN] 2^e of K rows
-  __half* vfac = reinterpret_cast<__half*>(kfac + (E4M3 ? FAC * BN : 0));  // [FAC][BN] 2^(e - emax) of V rows
-  int* vmax = reinterpret_cast<int*>(vfac + (E4M3 ? FAC * BN : 0));      // [FAC][4] emax of each tile
-  int* vexp = vmax + (E4M3 ? FAC * 4 : 0);                               // [MAX_NODES] exponents of the nodes' V
+  bf16* vlog = kfac + (E4M3 ? FAC * BN : 0);                             // [FAC][BN] e of V rows
+  int* vexp = reinterpret_cast<int*>(vlog + (E4M3 ? FAC * BN : 0));      // [MAX_NODES] exponents of the nodes' V
   uint8_t* sExp = reinterpret_cast<uint8_t*>(vexp + (E4M3 ? MAX_NODES : 0));  // [FAC][2][BN] exponent bytes
   float* xmax = reinterpret_cast<float*>(sExp + (E4M3 ? FAC * 2 * BN : 0));   // [2][2][BM]
   float* xsum = xmax + 2 * 2 * BM;                                            // [2][2][BM]
   float* xq = xsum + 2 * 2 * BM;                                              // [2][2][BM]
-  int* page_rows = reinterpret_cast<int*>(xq + 2 * 2 * BM);                 // [4][8] of the producer
+  float* xtop = xq + 2 * 2 * BM;                                              // [2][2][BM]
+  int* page_rows = reinterpret_cast<int*>(xtop + 2 * 2 * BM);               // [4][8] of the producer
   uint64_t* bars = reinterpret_cast<uint64_t*>(page_rows + 32);
   uint64_t* full = bars;             // [NK]
   uint64_t* empty = full + NK;       // [NK]
@@ -745,7 +749,7 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
         }
       }
       float m = -INFINITY, l = 0.f;  // reference maximum (log2) and this half's sum
-      int ev = 0;                    // reference exponent of V (e4m3)
+      float mp = -INFINITY;          // e4m3: that of score and V exponent, which P is relative to
       for (int t = p.t0; t < p.t1; ++t, ++n) {
         const int sb = n & 1, left = p.keys(t) - half * 64;
         const uint64_t mask = t == p.nt ? anc : left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
@@ -756,7 +760,7 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
         bool grow = false;
         const uint32_t scol = tmem + lane_off + C::S_COL + sb * BN + half * 64;
         const uint32_t kf = sm100::smem_u32(kfac + (n % FAC) * BN + half * 64);
-        const uint32_t vf = sm100::smem_u32(vfac + (n % FAC) * BN + half * 64);
+        const uint32_t vl = sm100::smem_u32(vlog + (n % FAC) * BN + half * 64);
         // 32 scores: read, K's scale (e4m3), mask
         auto scores = [&](int c0, float (&x)[32]) {
           sm100::tmem_ld32(scol + c0, x);
@@ -781,24 +785,21 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
               if (!(mk & (1u << c))) x[c] = -INFINITY;
           }
         };
-        float back = 1.f, shift = 0.f;  // this tile's V scale relative to the reference (e4m3)
-        if constexpr (E4M3) {
-          const int e = vmax[(n % FAC) * 4];
-          if (t == p.t0) ev = e;
-          if (e > ev + V_LAG) {
-            alpha_o = pow2(max(ev - e, -126));
-            ev = e;
-            grow = true;
+        // V's exponents of 8 keys
+        auto exponents = [&](int c, float (&f)[8]) {
+          const uint4 v4 = lds4(vl + c * 2);
+          const uint32_t w[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
           }
-          const int de = max(e - ev, -100);  // goes into the exponent, and out of the sum again
-          shift = (float)de;
-          back = pow2(-de);
-        }
+        };
         // maximum first, then P, each a loop over 32 scores. One pass over all 64 with a second one
         // when the maximum grew was slower: its code is fetched faster than the instruction cache
         // gives it (e4m3, 32 x 14000 keys, 21 nodes: 760 us, these loops 552).
         if (warp_on) {
-          float mt = -INFINITY;
+          float mt = -INFINITY, mpt = -INFINITY;
 #pragma unroll 1
           for (int c0 = 0; c0 < 64; c0 += 32) {
             float x[32];
@@ -807,15 +808,37 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
 #pragma unroll
             for (int c = 2; c < 32; ++c) mx[c & 1] = fmaxf(mx[c & 1], x[c]);
             mt = fmaxf(mt, fmaxf(mx[0], mx[1]));
+            if constexpr (E4M3) {
+              float px[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+              for (int c = 0; c < 32; c += 8) {
+                float ve[8];
+                exponents(c0 + c, ve);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) px[i & 1] = fmaxf(px[i & 1], fmaf(x[c + i], rs, ve[i]));
+              }
+              mpt = fmaxf(mpt, fmaxf(px[0], px[1]));
+            }
           }
+          if constexpr (E4M3) xtop[(sb * 2 + half) * BM + row] = mpt;  // exchanged with the next
           mt = fmaxf(mt, exchange(xmax + sb * 2 * BM, mt));
-          const float top = mt * rs - (E4M3 ? OFFSET8 : 0.f);
-          if (live && top > m + (E4M3 ? LAG8 : LAG)) {
+          const float top = mt * rs;
+          if (live && top > m + LAG) {
             const float f = sm100::exp2_approx(m - top);  // 0 on the first tile
-            alpha_o *= f;
             l *= f;
             m = top;
-            grow = true;
+            if constexpr (!E4M3) {
+              alpha_o = f;
+              grow = true;
+            }
+          }
+          if constexpr (E4M3) {
+            mpt = fmaxf(mpt, xtop[(sb * 2 + (half ^ 1)) * BM + row]);
+            if (live && mpt > mp + LAG8) {
+              alpha_o = sm100::exp2_approx(mp - mpt);
+              mp = mpt;
+              grow = true;
+            }
           }
         }
         // rescale O rows once the previous PV completed (warp-wide, rare after the first tiles)
@@ -832,30 +855,28 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
           }
         }
         if (warp_on) {
-          const float ref = (m == -INFINITY ? 0.f : m) - shift;
+          const float ref = m == -INFINITY ? 0.f : m;
+          const float ref_p = (mp == -INFINITY ? 0.f : mp) - OFFSET8;
           float sum[2] = {0.f, 0.f};
 #pragma unroll 1
           for (int c0 = 0; c0 < 64; c0 += 32) {
             float x[32];
             uint32_t pk[32];
             scores(c0, x);
-            uint4 vw[4];
-            if constexpr (E4M3) {
-#pragma unroll
-              for (int c = 0; c < 4; ++c) vw[c] = lds4(vf + (c0 + c * 8) * 2);
-            }
+            float ve[8];
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
+              if (E4M3 && c % 8 == 0) exponents(c0 + c, ve);
               float pr[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) pr[i] = sm100::exp2_approx(fmaf(x[c + i], rs, -ref));
               sum[0] += pr[0] + pr[1];
               sum[1] += pr[2] + pr[3];
               if constexpr (E4M3) {
-                const uint4 f = vw[c / 8];
-                const uint32_t f0 = c % 8 ? f.z : f.x, f1 = c % 8 ? f.w : f.y;
-                const __half2 h0 = __hmul2(__floats2half2_rn(pr[0], pr[1]), *reinterpret_cast<const __half2*>(&f0));
-                const __half2 h1 = __hmul2(__floats2half2_rn(pr[2], pr[3]), *reinterpret_cast<const __half2*>(&f1));
+#pragma unroll
+                for (int i = 0; i < 4; ++i)  // with V's scale: on its own range, whatever that of the sum is
+                  pr[i] = sm100::exp2_approx(fmaf(x[c + i], rs, ve[c % 8 + i]) - ref_p);
+                const __half2 h0 = __floats2half2_rn(pr[0], pr[1]), h1 = __floats2half2_rn(pr[2], pr[3]);
                 uint32_t w0 = *reinterpret_cast<const uint32_t*>(&h0), w1 = *reinterpret_cast<const uint32_t*>(&h1);
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {  // the high byte of an f16 is an e5m2
@@ -879,7 +900,7 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
             }
             sm100::tmem_st32_async(scol + c0, pk);  // over the scores just read
           }
-          l += (sum[0] + sum[1]) * back;
+          l += sum[0] + sum[1];
           sm100::tmem_st_wait();
         }
         sm100::tc_fence_before();
@@ -904,8 +925,10 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
       if (warp_on) {
         l += exchange(xsum + (pc & 1) * 2 * BM, l);
         // O -> the output (a whole segment) or the workspace
-        const float vs = E4M3 ? pow2(ev) : 1.f;
-        const float inv = l > 0.f ? vs / l : (l == 0.f ? 0.f : l);
+        // e4m3: O is relative to mp and OFFSET8, l to m. Two factors, since their product may leave the
+        // range of fp32 where the result does not.
+        const float inv = (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) * (E4M3 ? pow2(-(int)OFFSET8) : 1.f);
+        const float vs = !E4M3 ? 1.f : mp == -INFINITY ? 0.f : sm100::exp2_approx(mp - m);
         // a CTA has one part that begins a segment (slot 1) and one that goes on with one (0) at most
         const int slot = p.t0 == 0;
         const int64_t at = ((int64_t)blockIdx.x * 2 + slot) * rows + row;
@@ -927,7 +950,7 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
                 const uint32_t gg[4] = {gc[i / 8].x, gc[i / 8].y, gc[i / 8].z, gc[i / 8].w};
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
-                  float o0 = v[i + j] * inv, o1 = v[i + j + 1] * inv;
+                  float o0 = v[i + j] * inv * vs, o1 = v[i + j + 1] * inv * vs;
                   if (gated) {
                     o0 *= __fdividef(1.f, 1.f + __expf(-__uint_as_float(gg[j / 2] << 16)));
                     o1 *= __fdividef(1.f, 1.f + __expf(-__uint_as_float(gg[j / 2] & 0xffff0000u)));
@@ -943,7 +966,7 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
             for (int i = 0; i < 32; i += 4)
               if (c + i < a.D)
                 *reinterpret_cast<float4*>(a.part + at * a.D + c + i) =
-                    live ? make_float4(v[i] * vs, v[i + 1] * vs, v[i + 2] * vs, v[i + 3] * vs)
+                    live ? make_float4(v[i] * inv * vs, v[i + 1] * inv * vs, v[i + 2] * inv * vs, v[i + 3] * inv * vs)
                          : make_float4(0.f, 0.f, 0.f, 0.f);
           }
         }
@@ -987,19 +1010,12 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
             if (n >= FAC) wait_all(&f_free[fb], (n / FAC - 1) & 1);
             wait_all(&e_full[fb], (n / FAC) & 1);
             const uint8_t* ex = sExp + fb * 2 * BN;
-            int e[4], top = EXP_MIN;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int x = lane + 32 * i;
               kfac[fb * BN + x] = __float2bfloat16(x < keys ? pow2(min(max((int)ex[x] - EXP_BIAS, EXP_MIN), EXP_MAX)) : 0.f);
-              e[i] = min(max((int)ex[BN + x] - EXP_BIAS, EXP_MIN), EXP_MAX);
-              if (x < keys) top = max(top, e[i]);
+              vlog[fb * BN + x] = __float2bfloat16((float)min(max((int)ex[BN + x] - EXP_BIAS, EXP_MIN), EXP_MAX));
             }
-            top = __reduce_max_sync(0xffffffff, top);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              vfac[fb * BN + lane + 32 * i] = __float2half(lane + 32 * i < keys ? pow2(max(e[i] - top, -126)) : 0.f);
-            if (lane == 0) vmax[fb * 4] = top;
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive(&f_full[fb]);
           }
@@ -1057,15 +1073,13 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
         sm100::named_sync(5, CONV_WARPS * 32);
         if (cw == 0) {
           if (lane < DA) sm100::mbar_arrive(&full[(r0.st + lane) % NK]);
-          if (!pv) {  // V's factors relative to the largest
-            const int e0 = vexp[lane], e1 = vexp[lane + 32];
-            const int top = __reduce_max_sync(0xffffffff, max(lane < keys ? e0 : EXP_MIN, lane + 32 < keys ? e1 : EXP_MIN));
+          if (!pv) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              vfac[fb * BN + i * 32 + lane] = __float2half(i * 32 + lane < keys ? pow2(max((i ? e1 : e0) - top, -126)) : 0.f);
-              if (i >= 2) kfac[fb * BN + i * 32 + lane] = __float2bfloat16(0.f);
+              const int x = lane + 32 * i;
+              vlog[fb * BN + x] = __float2bfloat16(x < keys ? (float)vexp[x] : 0.f);
+              if (i >= 2) kfac[fb * BN + x] = __float2bfloat16(0.f);
             }
-            if (lane == 0) vmax[fb * 4] = top;
             __syncwarp();
             if (lane == 0) {
               sm100::mbar_arrive(&e_full[fb]);  // keeps its phase in step with the tiles
@@ -1112,8 +1126,8 @@ __global__ void __launch_bounds__(256) tree_join_kernel(Args a) {
     float w = 0.f;  // lane c: weight of part c0 + c
     if (c0 + lane < parts) {
       const float2 ml = a.ml[at(c0 + lane)];
-      w = ml.x == -INFINITY ? 0.f : sm100::exp2_approx(ml.x - top);
-      l = fmaf(w, ml.y, l);
+      w = ml.x == -INFINITY ? 0.f : sm100::exp2_approx(ml.x - top) * ml.y;
+      l += w;
     }
     const int n = min(32, parts - c0);
 #pragma unroll 4

@@ -146,6 +146,8 @@ def tree_attention(q, k, v, cache, table, lens, parents, counts=None, gate=None,
     Strided views are taken as they are when D is contiguous and rows are 16-byte aligned.
     Live nodes' k and v must be finite: a product with a masked one's zero probability is
     still formed. (Whatever lies in pages beyond ``lens`` or in padding nodes is not used.)
+    In a quantised cache, on the GPU, terms p_j v_j whose probability times V scale is below
+    2^-28 of the row's largest are dropped.
 
     Returns (out [b, T, Hq, D], lse [b, Hq, T] fp32, natural log, before the gate).
     """

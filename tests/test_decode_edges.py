@@ -6,7 +6,7 @@ import torch
 
 from nanospec_b200.ops import decode_ops as dops
 
-from test_decode_ops import BF, Delta, Problem, _device_error, devices, i32, near  # noqa: F401
+from test_decode_ops import BF, Delta, Problem, _device_error, devices, encode64, i32, near  # noqa: F401
 
 NARROW = [(2, 33, 1, 2, 16, None), (1, 64, 2, 1, 16, None), (2, 70, 2, 2, 16, [70, 41]), (2, 131, 1, 1, 16, [97, 131]),
           (1, 70, 1, 1, 32, None), (1, 70, 1, 1, 64, None)]
@@ -91,3 +91,80 @@ def test_out_states_that_overlap(dev):
             dops.gated_delta_advance(q, k, v, g, beta, a, 2, out_state=b)
         with pytest.raises(ValueError):
             dops.gated_delta_accept(k, g, u, path, a, 2, out_state=b)
+
+
+def rewrite(p, rows):
+    """Sequence 0's prefix of an e4m3 problem becomes rows [n, 2, Hk, D]."""
+    dev, page = p.args[0], p.cache.page_size
+    pos = torch.arange(len(rows))
+    slots = p.table[0].cpu()[pos // page].long() * page + pos % page
+    dops.cache_write(p.cache, rows[:, 0].to(dev), rows[:, 1].to(dev), slots.to(dev))
+    p.prefix[0] = encode64(rows)
+
+
+def aim(p, x):
+    """Channel 0 of every query is x."""
+    for q in (p.cpu[0], p.dev[0]):
+        q[..., 0] = x
+
+
+def scale_nodes(p, f):
+    """The nodes' V times f [T] (powers of two)."""
+    p.cpu[2] = (p.cpu[2].float() * f[None, :, None, None]).bfloat16()
+    p.dev[2] = p.cpu[2].to(p.args[0])
+
+
+@devices
+@pytest.mark.parametrize("far", [16, 22, 26, 30, 100])
+@pytest.mark.parametrize("n,b", [(128, 1), (400, 1), (400, 80)])
+def test_value_scale_of_a_key_without_weight(dev, far, n, b):
+    """One cached row of V is 2^far times the others', but its key has no probability."""
+    if b > 1 and dev == "cpu":
+        pytest.skip("the same statement as one sequence")
+    p = Problem(dev, [n] + [300] * (b - 1), 2, 4, 2, 64, 16, True, gate=False)
+    rows = torch.randn(n, 2, 2, 64).bfloat16()
+    rows[:, 0, :, 0] = 0
+    rows[5, 0, :, 0] = -160.0  # score -160 and e^-160 of the probability
+    rows[5, 1] *= 2.0 ** far
+    aim(p, 8.0)
+    rewrite(p, rows)
+    p.check(*p.run())
+
+
+@devices
+def test_value_scale_of_a_hidden_node(dev):
+    """A drafted node that others do not see has V of 2^30 times theirs."""
+    p = Problem(dev, [100], 4, 4, 2, 64, 16, True, gate=False)
+    p.parents = i32([[-1, 0, 0, 2]], "cpu")
+    scale_nodes(p, torch.tensor([1.0, 2.0 ** 30, 1.0, 1.0]))
+    p.check(*p.run())
+
+
+@devices
+@pytest.mark.parametrize("n", [500, 6000])
+def test_sink_without_value(dev, n):
+    """One key takes nearly all the probability and has V = 0: the others are the output."""
+    p = Problem(dev, [n], 1, 4, 2, 64, 16, True, gate=False)
+    rows = torch.randn(n, 2, 2, 64).bfloat16()
+    rows[:, 0] *= 0.25
+    rows[:, 0, :, 0] = 0
+    rows[3, 0, :, 0] = 17.0  # e^17 = 2^24.5 times the others' probability
+    rows[3, 1] = 0
+    aim(p, 8.0)
+    rewrite(p, rows)
+    p.check(*p.run())
+
+
+@devices
+def test_values_near_the_top_and_bottom(dev):
+    """V rows at the ends of the exponents' range."""
+    for e in (-110, 110):
+        p = Problem(dev, [300], 2, 4, 2, 64, 16, True, gate=False)
+        rows = torch.randn(300, 2, 2, 64).bfloat16()
+        rows[:, 1] *= 2.0 ** e
+        scale_nodes(p, torch.full((2,), 2.0 ** e))
+        rewrite(p, rows)
+        out, lse = p.run()
+        p.prefix[0][:, 1] *= 2.0 ** -e
+        p.cpu[2] = (p.cpu[2].float() * 2.0 ** -e).bfloat16()
+        p.check(out.float() * 2.0 ** -e, lse)
