@@ -1144,7 +1144,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(Args a) {
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffff, l, x);
   const bool live = tok < sequence(a, s, false).cnt;
-  const float inv = 1.f / l;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: every score was -inf
   if (on) {
     const uint32_t gg[4] = {gw.x, gw.y, gw.z, gw.w};
     uint32_t w[4];

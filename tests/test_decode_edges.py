@@ -1,6 +1,8 @@
 """Decoding ops where a size, an address, a scale or a value lies at an edge. Tolerances are those
 of test_decode_ops.py."""
 
+import math
+
 import pytest
 import torch
 
@@ -168,3 +170,36 @@ def test_values_near_the_top_and_bottom(dev):
         p.prefix[0][:, 1] *= 2.0 ** -e
         p.cpu[2] = (p.cpu[2].float() * 2.0 ** -e).bfloat16()
         p.check(out.float() * 2.0 ** -e, lse)
+
+
+@devices
+@pytest.mark.parametrize("far", [2, 3, 70, 110])
+@pytest.mark.parametrize("b", [1, 80])
+def test_value_scale_of_a_key_with_weight(dev, far, b):
+    """One cached row of V is 2^far times the others' and its key counts like any other; a
+    sequence per CTA, and several."""
+    if b > 1 and dev == "cpu":
+        pytest.skip("the same statement as one sequence")
+    p = Problem(dev, [400] + [300] * (b - 1), 2, 4, 2, 64, 16, True, gate=False)
+    rows = torch.randn(400, 2, 2, 64).bfloat16()
+    rows[:, 1].clamp_(-3, 3)
+    rows[:, 1, :, 1] = 3.0  # the same scale in every row
+    rows[5, 1] *= 2.0 ** far
+    rewrite(p, rows)
+    p.check(*p.run())
+
+
+@devices
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("n", [0, 700])
+def test_scores_that_overflow_downwards(dev, e4m3, n):
+    """Every score is -inf: zeros, lse -inf, however the keys are split."""
+    p = Problem(dev, [n], 1, 4, 2, 64, 64, e4m3, gate=False)
+    p.dev[0].fill_(3e38)
+    p.dev[1].fill_(-3e38)
+    if n:
+        rows = torch.randn(n, 2, 2, 64).bfloat16()
+        rows[:, 0] = -1e38
+        rewrite(p, rows)
+    out, lse = p.run()
+    assert (out == 0).all() and (lse == -math.inf).all()
