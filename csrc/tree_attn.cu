@@ -46,6 +46,8 @@
 // Rows of V beyond a sequence's end (stale pages, NaN) are zeroed in shared memory, since
 // 0 * NaN would reach O; masked scores are replaced, not added to. Every mbarrier wait is
 // bounded; a timeout sets the device error word and the kernel unwinds.
+#include <cfloat>
+
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
@@ -691,7 +693,8 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
       const bool in = row < rows && g < a.G && tok < a.T;
       const bool live = in && tok < p.q.cnt;
       const int hq = p.hk * a.G + g;
-      float rs = a.scale_log2;  // multiplies the products of this row
+      // multiplies the products of this row; never 0, which masked scores of -inf would turn into NaN
+      float rs = fmaxf(a.scale_log2, FLT_MIN);
       if constexpr (E4M3) {
         // q row -> e4m3 and e5m2 rows with a power-of-two scale (the previous piece's products are
         // complete: this thread has seen all of its scores); this thread's half
@@ -715,7 +718,7 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
           }
           top = max(top, __float_as_uint(exchange(xq + (pc & 1) * 2 * BM, __uint_as_float(top))));
           const int e = row_exponent(top, 7);
-          rs *= pow2(e);
+          rs = fmaxf(rs * pow2(e), FLT_MIN);
           const float sc = pow2(-e);
 #pragma unroll 1
           for (int c0 = 0; c0 < QC; c0 += 8) {

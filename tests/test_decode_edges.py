@@ -203,3 +203,14 @@ def test_scores_that_overflow_downwards(dev, e4m3, n):
         rewrite(p, rows)
     out, lse = p.run()
     assert (out == 0).all() and (lse == -math.inf).all()
+
+
+@devices
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("scale", [1e-30, 1e-60])
+def test_vanishing_scale(dev, e4m3, scale):
+    """Scores that vanish: the mean of what is seen."""
+    p = Problem(dev, [200], 3, 4, 2, 64, 64, e4m3, gate=False)
+    for q in (p.cpu[0], p.dev[0]):
+        q[:, 1] = 0
+    p.check(*p.run(scale=scale), scale=scale)
