@@ -284,13 +284,15 @@ __device__ __forceinline__ int row_exponent(uint32_t top, int at) {
   return max(min((int)(top >> 23) - 127 - at, EXP_MAX), EXP_MIN);
 }
 
-__device__ __forceinline__ uint32_t finite_top(uint4 w) {  // largest finite magnitude of 8 bf16
+// largest magnitude (its bits) of 8 bf16; infinities and NaN do not count, or are above all others
+template <bool FINITE>
+__device__ __forceinline__ uint32_t largest(uint4 w) {
   const uint32_t in[4] = {w.x, w.y, w.z, w.w};
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t lo = (in[i] << 16) & 0x7fffffffu, hi = in[i] & 0x7fff0000u;
-    top = max(top, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
+    top = max(top, max(!FINITE || lo < 0x7f800000u ? lo : 0u, !FINITE || hi < 0x7f800000u ? hi : 0u));
   }
   return top;
 }
@@ -714,11 +716,12 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
           for (int c0 = 0; c0 < QC; c0 += 8) {
             load(c0, w);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) top = max(top, finite_top(w[c]));
+            for (int c = 0; c < 8; ++c) top = max(top, largest<false>(w[c]));
           }
           top = max(top, __float_as_uint(exchange(xq + (pc & 1) * 2 * BM, __uint_as_float(top))));
           const int e = row_exponent(top, 7);
-          rs = fmaxf(rs * pow2(e), FLT_MIN);
+          // a row that is not finite has no finite score (e4m3 would saturate)
+          rs = top < 0x7f800000u ? fmaxf(rs * pow2(e), FLT_MIN) : NAN;
           const float sc = pow2(-e);
 #pragma unroll 1
           for (int c0 = 0; c0 < QC; c0 += 8) {
@@ -1054,8 +1057,8 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
             const int x = x0 + y * CONV_WARPS;
             int e;
             if (!pv) {  // exponents that bring the rows into [2^7, 2^8)
-              e = x < keys ? row_exponent(__reduce_max_sync(0xffffffff, finite_top(k4[y])), 7) : EXP_MIN;
-              const int ve = row_exponent(__reduce_max_sync(0xffffffff, finite_top(v4[y])), 7);
+              e = x < keys ? row_exponent(__reduce_max_sync(0xffffffff, largest<true>(k4[y])), 7) : EXP_MIN;
+              const int ve = row_exponent(__reduce_max_sync(0xffffffff, largest<true>(v4[y])), 7);
               if (lane == 0) {
                 kfac[fb * BN + x] = __float2bfloat16(x < keys ? pow2(e) : 0.f);
                 vexp[x] = x < keys ? ve : EXP_MIN;
@@ -1129,7 +1132,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(Args a) {
     float w = 0.f;  // lane c: weight of part c0 + c
     if (c0 + lane < parts) {
       const float2 ml = a.ml[at(c0 + lane)];
-      w = ml.x == -INFINITY ? 0.f : sm100::exp2_approx(ml.x - top) * ml.y;
+      w = ml.x == -INFINITY ? ml.y : sm100::exp2_approx(ml.x - top) * ml.y;  // (0, or NaN of a row that is)
       l += w;
     }
     const int n = min(32, parts - c0);

@@ -214,3 +214,17 @@ def test_vanishing_scale(dev, e4m3, scale):
     for q in (p.cpu[0], p.dev[0]):
         q[:, 1] = 0
     p.check(*p.run(scale=scale), scale=scale)
+
+
+@devices
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_queries_that_are_not_finite(dev, e4m3, bad):
+    """A query row that is not finite has no finite output, and leaves other rows alone."""
+    p = Problem(dev, [200], 3, 4, 2, 64, 64, e4m3, gate=False)
+    want = p.run()
+    p.dev[0][0, 1, 2, 7] = bad
+    out, lse = p.run()
+    assert not torch.isfinite(out[0, 1, 2]).any() and not torch.isfinite(lse[0, 2, 1])
+    out[0, 1, 2], lse[0, 2, 1] = want[0][0, 1, 2], want[1][0, 2, 1]
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
