@@ -1249,7 +1249,8 @@ std::vector<at::Tensor> tree_attention(at::Tensor q, at::Tensor k, at::Tensor v,
   NS_VALUE(table.device() == dev && table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == b &&
                table.is_contiguous(),
            "table must be contiguous int32 [b, max_pages]");
-  NS_VALUE(table.size(1) * c.page < (int64_t(1) << 31), "tree_attention: sequences of more than 2^31 rows");
+  // positions are 32-bit, those of the last tile's end included
+  NS_VALUE(table.size(1) * c.page <= (int64_t(1) << 31) - 2 * tattn::BN, "tree_attention: sequences of 2^31 rows");
   tattn::Args a{};
   a.lens = check_index(lens, b, dev, "lens");
   a.counts = check_index(counts, b, dev, "counts");

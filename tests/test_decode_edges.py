@@ -228,3 +228,14 @@ def test_queries_that_are_not_finite(dev, e4m3, bad):
     assert not torch.isfinite(out[0, 1, 2]).any() and not torch.isfinite(lse[0, 2, 1])
     out[0, 1, 2], lse[0, 2, 1] = want[0][0, 1, 2], want[1][0, 2, 1]
     assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dev", ["cuda"])
+def test_refuses_tables_beyond_32_bits(dev):
+    """Positions are counted in 32 bits, a tile beyond the last one included."""
+    cache = dops.PagedCache.allocate(2, 1, 128, 16, device=dev)
+    q = torch.zeros(1, 1, 1, 16, dtype=torch.bfloat16, device=dev)
+    table = torch.zeros(1, (1 << 24) - 1, dtype=torch.int32, device=dev)
+    with pytest.raises(ValueError):
+        dops.tree_attention(q, q, q, cache, table, i32([100], dev), i32([-1], dev))
