@@ -1238,7 +1238,7 @@ std::vector<at::Tensor> tree_attention(at::Tensor q, at::Tensor k, at::Tensor v,
                  x->size(1) == T && x->size(2) == c.heads && x->size(3) == c.d,
              "tree_attention: k and v must be bfloat16 [b, T, Hk, D] like the cache");
   NS_VALUE(D == c.d, "tree_attention: q and the cache differ in head_dim");
-  NS_VALUE(Hq >= 1 && Hq % c.heads == 0, "tree_attention: query heads must be a multiple of key heads");
+  NS_VALUE(Hq >= 1 && c.heads >= 1 && Hq % c.heads == 0, "tree_attention: query heads must be a multiple of key heads");
   NS_VALUE(T >= 1 && T <= MAX_NODES, "a tree has 1 to 64 nodes");
   NS_VALUE(c.pages >= 1, "tree_attention: the cache has no pages");
   NS_VALUE(!gate.has_value() || (gate->sizes() == q.sizes() && gate->scalar_type() == at::kBFloat16 &&

@@ -157,7 +157,7 @@ def tree_attention(q, k, v, cache, table, lens, parents, counts=None, gate=None,
     b, t, hq, d = q.shape
     _need(k.shape == v.shape == (b, t, cache.k.shape[1], cache.k.shape[3]) and d == cache.k.shape[3],
           "tree_attention: k and v must be [b, T, Hk, D] like the cache")
-    _need(hq % k.shape[2] == 0, "tree_attention: query heads must be a multiple of key heads")
+    _need(hq >= 1 and k.shape[2] >= 1 and hq % k.shape[2] == 0, "tree_attention: query heads must be a multiple of key heads")
     _need(gate is None or gate.shape == q.shape, "tree_attention: gate must have q's shape")
     _need(scale is None or scale > 0, "tree_attention: scale must be positive")
     _check_table(cache, table, lens)

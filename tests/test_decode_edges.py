@@ -239,3 +239,11 @@ def test_refuses_tables_beyond_32_bits(dev):
     table = torch.zeros(1, (1 << 24) - 1, dtype=torch.int32, device=dev)
     with pytest.raises(ValueError):
         dops.tree_attention(q, q, q, cache, table, i32([100], dev), i32([-1], dev))
+
+
+@devices
+def test_refuses_no_key_heads(dev):
+    z = lambda h: torch.zeros(1, 1, h, 64, dtype=torch.bfloat16, device=dev)  # noqa: E731
+    cache = dops.PagedCache.allocate(2, 0, 16, 64, device=dev)
+    with pytest.raises(ValueError):
+        dops.tree_attention(z(4), z(0), z(0), cache, i32([[0]], dev), i32([3], dev), i32([-1], dev))
