@@ -39,6 +39,23 @@ def tree_depths(parents):
     return depth.view_as(parents)
 
 
+def path_end(parents, path):
+    """Last node (-1: none) of every row of path [b, m], which must be a way down the tree
+    parents [b, T]: root first, each node the child of the one before, -1 skipped. On the CPU."""
+    b, t = parents.shape
+    if path.dim() != 2 or path.shape[0] != b or path.is_floating_point():
+        raise ValueError("nanospec_b200: path must be integers [b, m], a row per sequence")
+    if path.shape[1] > dops.MAX_NODES or bool(((path < -1) | (path >= t)).any()):
+        raise ValueError("nanospec_b200: path must name nodes of the last tree, or -1")
+    last = torch.full((b,), -1, dtype=torch.int64)
+    for node in path.long().unbind(1):
+        up = parents.gather(1, node.clamp_min(0)[:, None])[:, 0]
+        if bool(((node >= 0) & (up != last)).any()):
+            raise ValueError("nanospec_b200: path must lead from the last cached token down the tree")
+        last = torch.where(node >= 0, node, last)
+    return last
+
+
 def greedy_path(tokens, parents, logits):
     """The nodes that greedy decoding keeps, and its next token.
 
@@ -126,8 +143,8 @@ class DecodeSession:
         depth = tree_depths(parents).expand(b, t)
         self._fit(int(depth.max()) + 1)
         dev = self.device
-        par = parents.to(torch.int32).expand(b, t).contiguous()
-        step = dict(depth=depth, parents=par.to(dev), lens=self.lens.to(dev), windows=self._windows(par), layers={})
+        par = parents.to(torch.int32).expand(b, t).clone(memory_format=torch.contiguous_format)  # kept until accept()
+        step = dict(tree=par, parents=par.to(dev), lens=self.lens.to(dev), windows=self._windows(par), layers={})
         x = self._run(tokens, self.lens[:, None] + depth, lambda i, attn, n: self._tree_gdn(step, i, attn, n),
                       lambda i, attn, qg, k, v, cos, sin: self._tree_attention(step, i, attn, qg, k, v, cos, sin))
         self.pending = step
@@ -135,15 +152,18 @@ class DecodeSession:
 
     @torch.no_grad()
     def accept(self, path):
-        """Keep the nodes ``path`` [b, m] (CPU int32, root first, -1 padding) of the last tree."""
+        """Keep the nodes ``path`` [b, m] (on the CPU, root first, -1 padding) of the last tree.
+
+        Every row's nodes must be a way down from the last cached token (each the child of the
+        one before); anything else raises ``ValueError`` and changes nothing.
+        """
         step = self.pending
         if step is None:
             raise ValueError("nanospec_b200: accept() follows verify()")
-        b, m = path.shape
-        t = step["depth"].shape[1]
-        if b != self.batch or bool((path >= t).any()):
-            raise ValueError("nanospec_b200: path must name nodes of the last tree")
+        last = path_end(step["tree"], path)
+        path = path.to(torch.int32).contiguous()
         self.pending = None
+        b = path.shape[0]
         on = path >= 0
         # slots of the kept nodes: positions after the cached ones, in the order of the path
         at = self.lens[:, None].long() + on.long().cumsum(1) - 1
@@ -152,7 +172,6 @@ class DecodeSession:
         dpath = path.to(self.device)
         rows = torch.arange(b, device=self.device)[:, None]
         # the convolution's inputs end with the last kept node (its window is the new tail)
-        last = torch.where(on.any(1), path.gather(1, (on.long().cumsum(1).argmax(1))[:, None])[:, 0].long(), -1)
         tail = self._tail(step["windows"], last).to(self.device)
         for i, keep in step["layers"].items():
             if i in self.caches:

@@ -6,6 +6,8 @@ import math
 import pytest
 import torch
 
+from nanospec_b200 import decode
+from nanospec_b200.models import verifier as V
 from nanospec_b200.ops import decode_ops as dops
 
 from test_decode_ops import BF, Delta, Problem, _device_error, devices, encode64, i32, near  # noqa: F401
@@ -247,3 +249,45 @@ def test_refuses_no_key_heads(dev):
     cache = dops.PagedCache.allocate(2, 0, 16, 64, device=dev)
     with pytest.raises(ValueError):
         dops.tree_attention(z(4), z(0), z(0), cache, i32([[0]], dev), i32([3], dev), i32([-1], dev))
+
+
+STAGE = {}
+
+
+def stage_of(dev, kernel=4):
+    if dev == "cuda" and not torch.cuda.is_available():
+        pytest.skip("needs a CUDA GPU")
+    if (dev, kernel) not in STAGE:
+        dtype = torch.bfloat16 if dev == "cuda" else torch.float32
+        tc = V.tiny_hybrid_text_config(head_dim=32)
+        tc["linear_conv_kernel_dim"] = kernel
+        w = V.random_verifier_weights(tc, 0, 4, device="cpu", first=True, last=True, seed=1, std=0.15, dtype=dtype)
+        STAGE[dev, kernel] = V.QwenStage(None, 0, 4, device=dev, first=True, last=True,
+                                         weights={k: v.to(dev) for k, v in w.items()}, config=V.synthetic_hf_config(tc))
+    return STAGE[dev, kernel]
+
+
+def snapshot(s):
+    return ([x.clone() for c in s.caches.values() for x in (c.k.view(torch.uint8), c.v.view(torch.uint8))]
+            + [x.clone() for x in s.states.values()] + [x.clone() for x in s.convs.values()] + [s.lens.clone()])
+
+
+@devices
+def test_accept_refuses_what_is_no_path(dev):
+    """Siblings, skipped or repeated ancestors, entries below -1: nothing changes, in particular
+    not the next sequence's pages."""
+    s = decode.DecodeSession(stage_of(dev), 2, 16, page_size=16)
+    s.prompt(torch.zeros(2, 8, dtype=torch.int64))
+    parents = i32([-1, 0, 0, 1], "cpu")
+    s.verify(torch.zeros(2, 4, dtype=torch.int64), parents)
+    before = snapshot(s)
+    good = [0, 1, 3]
+    for bad in ([1], [0, 3], [0, 0], [0, 1, 2], [0, -2], [4], [1, 0], [0] * 9, [0, 2, 3]):
+        n = max(len(bad), 3)
+        rows = [good + [-1] * (n - 3), bad + [-1] * (n - len(bad))]
+        with pytest.raises(ValueError):
+            s.accept(i32(rows, "cpu"))
+        assert all(torch.equal(a, b) for a, b in zip(before, snapshot(s)))
+    parents.fill_(-1)  # the session has its own
+    s.accept(torch.tensor([[0, 0], [1, 2], [3, -1]]).T)  # the tree is still there; any integer type and strides will do
+    assert s.lens.tolist() == [11, 10]
