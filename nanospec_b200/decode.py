@@ -127,6 +127,7 @@ class DecodeSession:
             raise ValueError("nanospec_b200: prompt() fills an empty session, one row per sequence")
         b, s = ids.shape
         self._fit(s)
+        self.pending = None  # a tree over the empty session is none of this prompt's
         pos = torch.arange(s).expand(b, s)
         x = self._run(ids, pos, lambda i, attn, n: self._prompt_gdn(i, attn, n),
                       lambda i, attn, qg, k, v, cos, sin: self._prompt_attention(i, attn, qg, k, v, cos, sin))

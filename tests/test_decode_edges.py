@@ -291,3 +291,11 @@ def test_accept_refuses_what_is_no_path(dev):
     parents.fill_(-1)  # the session has its own
     s.accept(torch.tensor([[0, 0], [1, 2], [3, -1]]).T)  # the tree is still there; any integer type and strides will do
     assert s.lens.tolist() == [11, 10]
+
+
+def test_prompt_drops_the_last_tree():
+    s = decode.DecodeSession(stage_of("cpu"), 1, 32)
+    s.verify(torch.zeros(1, 2, dtype=torch.int64), i32([-1, 0], "cpu"))
+    s.prompt(torch.zeros(1, 8, dtype=torch.int64))
+    with pytest.raises(ValueError):
+        s.accept(i32([[0, 1]], "cpu"))
