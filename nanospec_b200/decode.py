@@ -233,7 +233,7 @@ class DecodeSession:
         mixed, z, g, beta = self._project(attn, n)
         q, k, v, groups = self._heads(attn, vops.causal_conv_silu(mixed, attn.conv1d.weight))
         out, _ = dops.gated_delta_advance(q, k, v, g, beta, self.states[i], groups)
-        self.convs[i] = torch.cat((self.convs[i], mixed), 1)[:, -self.convs[i].shape[1]:].contiguous()
+        self.convs[i] = torch.cat((self.convs[i], mixed), 1)[:, mixed.shape[1]:].contiguous()
         return self._output(attn, out, z)
 
     def _tree_gdn(self, step, i, attn, n):

@@ -299,3 +299,21 @@ def test_prompt_drops_the_last_tree():
     s.prompt(torch.zeros(1, 8, dtype=torch.int64))
     with pytest.raises(ValueError):
         s.accept(i32([[0, 1]], "cpu"))
+
+
+@devices
+def test_session_without_convolution_history(dev):
+    """A convolution of width 1 keeps no inputs."""
+    stage = stage_of(dev, kernel=1)
+    gen = torch.Generator().manual_seed(2)
+    ids = torch.randint(0, stage.config["vocab_size"], (1, 12), generator=gen)
+    s = decode.DecodeSession(stage, 1, 64, quantize=False)
+    s.prompt(ids[:, :8])
+    for i in range(8, 12):
+        logits = s.verify(ids[:, i:i + 1], i32([-1], "cpu"))
+        s.accept(i32([[0]], "cpu"))
+    assert all(c.shape[1] == 0 for c in s.convs.values())
+    x, _ = V.stage_forward(stage, ids.to(dev))
+    want = (x.float() @ stage.lm_head.weight.float().T).cpu()[0, -1]
+    got = logits[0, 0].float().cpu()
+    assert torch.nn.functional.cosine_similarity(got, want, dim=0) > (0.99 if dev == "cuda" else 0.99999)
