@@ -27,9 +27,10 @@
 // solved by blocks of 16 nodes in fp32.
 //
 // Measured (48 heads of 128): one token of 64 sequences 75 us and short paths 76 us (5.4 TB/s,
-// 84 % of the copy rate), the states' bytes. Trees: 16 sequences x 16 nodes 42 us, 32 x 61 nodes
-// 244 us (0.9 TB/s): a CTA's phases wait for one another (loads, S K, M, solve, A u) with 12
-// warps an SM to hide it, 3 CTAs by registers.
+// 84 % of the copy rate), the states' bytes. Trees: 16 sequences x 16 nodes 44 us, 32 x 61 nodes
+// 224 us (0.95 TB/s); 333 tokens of 2 sequences 132 us, six chunks in a row. A CTA's phases wait
+// for one another (loads, S K, M, solve, A u) with few warps an SM to hide it: 12 up to 32 nodes (3
+// CTAs by registers), 8 beyond (2 by shared memory; kept to the 168 registers of three, 243 and 156 us).
 #include "decode.h"
 #include "sm100.cuh"
 
@@ -215,12 +216,16 @@ struct Nodes {
   static constexpr int AS = TP + 8;                    // words of a row of node pairs (8 banks apart)
   static constexpr int ROWS = TP * KST * 2;            // bytes of K or Q
   static constexpr int SMEM = 2 * ROWS + TP * US * 4 + TP * MS * 4 + TP * AS * 4 + 8 * TP * 4;
+  // CTAs an SM that registers are kept for (three leave each of 128 threads 168, two 255): no more than an SM's
+  // 228 KB of shared memory holds, each with the 1 KB that the system takes
+  static constexpr int CTAS = 3 * (SMEM + 1024) <= 228 * 1024 ? 3 : 2;
+  static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory");
 };
 
 // TREE: T <= 8 NT nodes with parents; the state is only read. Otherwise tokens in chunks of
 // 8 NT whose state moves on.
 template <int D, int NT, bool TREE>
-__global__ void __launch_bounds__(Nodes<D, NT>::THREADS, 3) gdn_nodes_kernel(Args a) {
+__global__ void __launch_bounds__(Nodes<D, NT>::THREADS, Nodes<D, NT>::CTAS) gdn_nodes_kernel(Args a) {
   using C = Nodes<D, NT>;
   constexpr int TP = C::TP, TN = 8 * NT, KST = C::KST, US = C::US, MS = C::MS, AS = C::AS, COLS = C::COLS, SL = D / COLS;
   extern __shared__ __align__(16) uint8_t sm[];
