@@ -181,8 +181,8 @@ struct Walk {
   }
 };
 
-// First position and end of CTA blockIdx.x (warp-wide); total tiles in U, working CTAs in N
-// (each has a tile at least).
+// First position and end of CTA blockIdx.x (warp-wide); total units in U, CTAs that have any in N. A
+// run may lie wholly within a segment's first `seg` units: such a CTA has no tile and leaves no part.
 __device__ __forceinline__ Walk plan(const Args& a, int lane, int64_t& U, int& N) {
   int64_t sum = 0, n = 0;
   Seq q{0, 0};

@@ -251,6 +251,15 @@ def test_refuses_no_key_heads(dev):
         dops.tree_attention(z(4), z(0), z(0), cache, i32([[0]], dev), i32([3], dev), i32([-1], dev))
 
 
+@devices
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("n", [0, 1, 129])
+def test_less_work_than_processors(dev, e4m3, n):
+    """Fewer units of work than SMs: some blocks get no tile, every tile has a block of its own."""
+    p = Problem(dev, [n], 1, 1, 1, 128, 16, e4m3)
+    p.check(*p.run())
+
+
 STAGE = {}
 
 
