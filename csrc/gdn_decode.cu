@@ -683,6 +683,9 @@ __global__ void __launch_bounds__(Slice<D>::WARPS * 32) gdn_step_kernel(Args a, 
   }
 }
 
+// Up to here (of a batch's longest path) nodes one by one, beyond in blocks of 16 on tensor cores.
+// Measured, 64 sequences (us, one by one and in blocks): paths of 1 to m nodes 70 and 91 at m =
+// 4, 86 and 96 at 12, 96 and 98 at 16; all of m nodes 79 and 92 at 4, 99 and 95 at 8, 139 and 107 at 16.
 constexpr int SHORT_PATH = 16;
 
 template <int D>

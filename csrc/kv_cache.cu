@@ -10,10 +10,12 @@
 // only rounding is e4m3's own. e follows from the bits of a: a = 1.m * 2^E needs e = E - 8
 // when 1.m <= 1.75 (448 = 1.75 * 2^8) and E - 7 otherwise.
 //
-// Both kernels move each byte once and are bound by HBM: 16 channels per thread (16 bytes of
-// codes, 32 of bf16), index arithmetic in 32 bits with shifts, several rows' loads under way.
-// Writing 12288 rows x 8 heads x 128 as e4m3 and reading 33147 back: 98 us, 2.9 TB/s
-// (one 8-channel thread per element group with 64-bit divisions: 338 us).
+// Both kernels move each byte once: 16 channels per thread (16 bytes of codes, 32 of bf16), index
+// arithmetic in 32 bits with shifts, several rows' loads under way. Writing 12288 rows x 8 heads x
+// 128 as e4m3 and reading 33147 back: 99 us, 2.8 TB/s (one 8-channel thread per element group
+// with 64-bit divisions: 338 us). Less than half the copy rate: neighbouring threads take the heads
+// of one position, whose rows lie in different runs of the pages (a head's rows of one page adjoin),
+// and the arguments are indexed by block, so each thread holds a copy in local memory.
 #include <cuda_fp8.h>
 
 #include "decode.h"

@@ -38,10 +38,12 @@
 // rounding of the output at 2^18 such keys), the others keep 11 bits. The nodes' own
 // K and V are split like q. So no operand is converted on its way to the tensor cores.
 //
-// Measured (32 sequences of 14000 keys, 4 key heads of 256, pages of 64): bf16 390 us at one
-// node (4.71 TB/s) and 428 at 21 (541 TFLOP/s of products, 4.36 TB/s); e4m3 548 and 552 us
-// (1.7 TB/s). bf16 waits for K tiles at 73 % of the copy rate; e4m3 for its issuing and softmax
-// warps, whose work per tile is that of bf16 at half the bytes.
+// Measured (32 sequences of 14000 keys, 4 key heads of 256, pages of 64): bf16 378 us at one
+// node (4.86 TB/s) and 413 at 21 (561 TFLOP/s of products, 4.51 TB/s); e4m3 587 and 597 us
+// (1.6 TB/s). bf16 waits for K tiles at 75 % of the copy rate. e4m3 is bound by neither its products
+// nor its softmax: a quarter of the products with P takes 2 % less, half of the softmax 7 %, so
+// mostly by the steps of a tile waiting for one another. (Counting V's scale with the score
+// is 8 % of it: 548 and 552 us with V relative to the largest scale seen, which lost rows.)
 //
 // Rows of V beyond a sequence's end (stale pages, NaN) are zeroed in shared memory, since
 // 0 * NaN would reach O; masked scores are replaced, not added to. Every mbarrier wait is
@@ -803,7 +805,8 @@ __global__ void __launch_bounds__(Cfg<DT, E4M3>::THREADS, 1)
         };
         // maximum first, then P, each a loop over 32 scores. One pass over all 64 with a second one
         // when the maximum grew was slower: its code is fetched faster than the instruction cache
-        // gives it (e4m3, 32 x 14000 keys, 21 nodes: 760 us, these loops 552).
+        // gives it (e4m3, 32 x 14000 keys, 21 nodes, before V's scale counted with the score: 760
+        // us, these loops 552).
         if (warp_on) {
           float mt = -INFINITY, mpt = -INFINITY;
 #pragma unroll 1
@@ -1278,8 +1281,8 @@ std::vector<at::Tensor> tree_attention(at::Tensor q, at::Tensor k, at::Tensor v,
   a.pages = c.pages, a.max_pages = table.size(1);
   a.b = (int)b, a.T = (int)T, a.Hq = (int)Hq, a.Hk = c.heads, a.D = (int)D, a.page = c.page;
   a.page_log2 = c.page == 16 ? 4 : c.page == 32 ? 5 : c.page == 64 ? 6 : 7;
-  // measured at 2 and 4 (us): e4m3, one node of 64 ragged sequences, 479 and 448, bf16 short
-  // trees 65 and 72; an e4m3 segment also splits the nodes' rows
+  // measured at 2 and 4 (us): e4m3, one node of 64 ragged sequences, 522 and 487, bf16 short
+  // trees 66 and 71 (71 at 1 too); an e4m3 segment also splits the nodes' rows
   a.seg = c.e4m3 ? 4 : 2;
   a.G = (int)Hq / c.heads;
   a.HB = (a.G + tattn::BM - 1) / tattn::BM;

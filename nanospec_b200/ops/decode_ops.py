@@ -199,6 +199,8 @@ def gated_delta_verify(q, k, v, g, beta, state, parents, groups=1, counts=None, 
     Arguments as in ``gated_delta_advance`` and ``tree_attention``: node t continues from
     the state of node parents[t] (-1: ``state``). Returns (out [b, T, nv, D], u fp32
     [b, T, nv, D]); u holds the rows that the nodes would add, for ``gated_delta_accept``.
+    Live nodes' inputs must be finite (g may be -inf): on the GPU a node that is not an
+    ancestor is multiplied by zero. Padding nodes are not used.
     """
     if q.is_cuda:
         return _c().gdn_verify(q, k, v, g, beta, state, parents, int(groups), counts, rows)
